@@ -48,6 +48,13 @@ SIGNATURES = {
     "ekv_page_stats_init": (C.c_int, [_D, _I, _P]),
     "ekv_append": (C.c_int, [_D, _P, _P, _L, _L, _P, _P, _P]),
     "ekv_append_static": (C.c_int, [_D, _P, _P, _L, _L, _P, _P]),
+    "ekv_extend": (C.c_int, [_D, _P, _P, _L, _L, _L, _I, _P, _P, _L, _P, _P, _P, _P]),
+    "ekv_plan_block_tables": (C.c_int, [_P, _P, _I, _I, _I, _P, _L, _I, _P, _I, _P, _P, _I, _P, _P, _P]),
+    "ekv_release_blocks": (C.c_int, [_P, _P, _I, _I, _I, _P, _L, _I, _P, _I, _P, _P]),
+    "ekv_qk_norm_rope": (C.c_int, [_I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _L, _L, _P, _I, _I,
+                                   _P, _P, _I, _I, _F, _P]),
+    "ekv_tree_workspace_bytes": (_Z, [_D, _I, _I, _I]),
+    "ekv_tree_decode": (C.c_int, [_D, _P, _P, _I, _I, _P, _P, _P, _P, _P, _L, _L, _P, _I, _F, _P, _P, _P, _P, _Z, _P, _P]),
     "ekv_topk_select": (C.c_int, [_D, _P, _L, _L, _I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _L, _L, _P, _P]),
     "ekv_copy_timeouts": (C.c_int, [_P]),
     "ekv_topk_decode_stream_supported": (C.c_int, [_D, _I, _I, _I, _I]),
@@ -157,7 +164,29 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which the device of ``t`` is the current one: streams and launches belong to the current device."""
+    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 def require_cuda(*tensors) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError("entmaxkv_b200 runs on CUDA tensors only (sm_100a); got a CPU tensor")
+
+
+def require_same_device(device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"all tensors must be on {device}; got one on {t.device}")

@@ -1,0 +1,225 @@
+// Block tables and slot maps of a batch of requests, built on the GPU from their lengths.
+//
+// Sequence b holds ceil(seq[b] / P) pages and after this step's new[b] tokens needs ceil((seq[b] + new[b]) / P).  The
+// free list is a stack whose lowest sum(held) entries are in use, so its top needs no counter of its own: the pages
+// that the batch lacks take the entries from there on, in sequence order.  Nothing but the lengths is state, hence a
+// plan can be made twice (or made and dropped) with the same result.
+//
+// Everything is a prefix sum over the sequences.  Each thread block computes both prefix sums (tokens, pages) whole, in
+// shared memory, and then takes its share of the tokens and of the fresh pages, found by binary search: one launch, no
+// block waits for another.  Bound by latency for a decode step, by the slot stores for a batch of prompts.
+#include "ekv_common.cuh"
+
+namespace ekv {
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanMaxBatch = EKV_PLAN_MAX_BATCH;
+
+struct PlanArgs {
+  const int* seq;
+  const int* add;        // new tokens, or (release) tokens kept
+  int add_all;           // where add is null
+  int batch, page_size;
+  int* table;
+  int64_t table_stride;
+  int width;
+  int* free_list;
+  int n_free;
+  int64_t* slots;
+  int* positions;
+  int n_slots;
+  int* row_starts;
+  int* status;
+};
+
+// sums saturate: lengths are device data and may be anything, and a saturated sum still lies behind every buffer
+__device__ __forceinline__ int sat_add(int a, int b) {
+  return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu);
+}
+__device__ __forceinline__ int pages_of(int tokens, int P) { return tokens / P + (tokens % P ? 1 : 0); }
+
+struct SeqPages {
+  int seq, add, held, more;   // tokens, tokens added, pages held (after a release: kept), pages more (released)
+};
+template <bool RELEASE>
+__device__ __forceinline__ SeqPages seq_pages(const PlanArgs& a, int b) {
+  SeqPages s;
+  s.seq = max(a.seq[b], 0);
+  s.add = max(a.add ? a.add[b] : a.add_all, 0);
+  if (RELEASE) {
+    s.add = min(s.add, s.seq);
+    s.held = pages_of(s.add, a.page_size);
+    s.more = pages_of(s.seq, a.page_size) - s.held;
+  } else {
+    s.held = pages_of(s.seq, a.page_size);
+    s.more = pages_of(sat_add(s.seq, s.add), a.page_size) - s.held;
+  }
+  return s;
+}
+
+// inclusive saturating scan over the block's threads; also the total
+__device__ __forceinline__ int block_scan_sat(int v, int* scratch, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = sat_add(v, n);
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = v;
+  __syncthreads();
+  int base = 0, all = 0;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    const int s = scratch[w];
+    if (w < warp) base = sat_add(base, s);
+    all = sat_add(all, s);
+  }
+  *total = all;
+  return sat_add(base, v);
+}
+
+// first index whose (inclusive) prefix sum lies above x
+__device__ __forceinline__ int row_of(const int* ends, int n, int x) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ends[mid] > x) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
+template <bool RELEASE>
+__global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const __grid_constant__ PlanArgs a) {
+  extern __shared__ int s_ends[];          // [2][batch]: tokens, pages (inclusive prefix sums)
+  __shared__ int scratch[kPlanThreads / 32];
+  int* const tok_end = s_ends;
+  int* const page_end = s_ends + a.batch;
+  const int P = a.page_size, B = a.batch;
+  const int per = (B + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = min(threadIdx.x * per, B), b1 = min(b0 + per, B);
+  int tokens = 0, pages = 0, held = 0;
+  for (int b = b0; b < b1; ++b) {
+    const SeqPages s = seq_pages<RELEASE>(a, b);
+    tokens = sat_add(tokens, s.add);
+    pages = sat_add(pages, s.more);
+    held = sat_add(held, s.held);
+    tok_end[b] = tokens;
+    page_end[b] = pages;
+  }
+  int all_tokens, all_pages, head;
+  const int tok_incl = block_scan_sat(tokens, scratch, &all_tokens);
+  const int page_incl = block_scan_sat(pages, scratch, &all_pages);
+  block_scan_sat(held, scratch, &head);
+  // a saturated sum minus its last term would be wrong, but then everything behind it is out of range anyway
+  for (int b = b0; b < b1; ++b) {
+    tok_end[b] = sat_add(tok_end[b], tok_incl - tokens);
+    page_end[b] = sat_add(page_end[b], page_incl - pages);
+  }
+  __syncthreads();
+
+  const int first = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
+  for (int64_t f = first; f < all_pages; f += step) {
+    const int b = row_of(page_end, B, (int)f);
+    if (b >= B) break;
+    const SeqPages s = seq_pages<RELEASE>(a, b);
+    const int64_t p = (int64_t)s.held + (f - (page_end[b] - s.more));
+    if (p < 0 || p >= a.width) {
+      if (a.status) atomicOr(a.status, EKV_STATUS_CAPACITY);
+      continue;
+    }
+    int* const entry = a.table + b * a.table_stride + p;
+    const int64_t place = (int64_t)head + f;
+    const bool have = place < a.n_free;
+    if (RELEASE) {
+      const int block = *entry;
+      const bool ok = have && (unsigned)block < (unsigned)a.n_free;
+      if (ok) a.free_list[place] = block;
+      if (!ok && a.status) atomicOr(a.status, EKV_STATUS_PAGE_RANGE);
+      *entry = -1;
+    } else {
+      *entry = have ? a.free_list[place] : -1;
+      if (!have && a.status) atomicOr(a.status, EKV_STATUS_CAPACITY);
+    }
+  }
+  if (RELEASE) return;
+
+  if (a.row_starts)
+    for (int b = first; b <= B; b += step) a.row_starts[b] = b ? tok_end[b - 1] : 0;
+  if (a.slots || a.positions)
+    for (int64_t r = first; r < a.n_slots; r += step) {
+      int64_t slot = -1;
+      int pos = -1;
+      const int b = row_of(tok_end, B, (int)r);
+      if (b < B) {
+        const SeqPages s = seq_pages<false>(a, b);
+        pos = sat_add(s.seq, (int)r - (tok_end[b] - s.add));
+        const int p = pos / P;
+        int block = -1;
+        if (p < a.width) {
+          if (p < s.held) {
+            block = a.table[b * a.table_stride + p];
+          } else {      // taken in this launch, maybe by another block: the entry's value, not the entry
+            const int64_t place = (int64_t)head + (page_end[b] - s.more) + (p - s.held);
+            if (place < a.n_free) block = a.free_list[place];
+          }
+        }
+        if (block >= 0) slot = (int64_t)block * P + pos % P;
+      }
+      if (a.slots) a.slots[r] = slot;
+      if (a.positions) a.positions[r] = pos;
+    }
+}
+
+static int plan_check(const PlanArgs& a) {
+  if (a.batch < 0 || a.batch > kPlanMaxBatch || a.page_size <= 0 || a.width < 0 || a.n_free < 0 || a.n_slots < 0)
+    return EKV_ERR_ARG;
+  if (a.batch > 0 && (!a.seq || (a.width > 0 && !a.table) || (a.n_free > 0 && !a.free_list) || a.table_stride < a.width))
+    return EKV_ERR_ARG;
+  return EKV_OK;
+}
+
+template <bool RELEASE>
+static int plan_launch(const PlanArgs& a, int blocks, void* stream) {
+  const size_t smem = 2 * sizeof(int) * (size_t)a.batch;
+  if (smem > 40 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(plan_blocks_kernel<RELEASE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         2 * (int)sizeof(int) * kPlanMaxBatch);
+    if (e != cudaSuccess) return (int)e;
+  }
+  plan_blocks_kernel<RELEASE><<<blocks, kPlanThreads, smem, as_stream(stream)>>>(a);
+  return launch_status();
+}
+
+}  // namespace ekv
+
+extern "C" int ekv_plan_block_tables(const int32_t* seq_lens, const int32_t* new_lens, int32_t new_all, int32_t batch,
+                                     int32_t page_size, int32_t* block_table, int64_t bt_stride, int32_t width,
+                                     const int32_t* free_blocks, int32_t n_free, int64_t* slots, int32_t* positions,
+                                     int32_t n_slots, int32_t* row_starts, int32_t* status, void* stream) {
+  using namespace ekv;
+  PlanArgs a{seq_lens, new_lens, new_all, batch, page_size, block_table, bt_stride, width,
+             const_cast<int32_t*>(free_blocks), n_free, slots, positions, n_slots, row_starts, status};
+  if (int e = plan_check(a)) return e;
+  if (batch == 0 && n_slots == 0 && !row_starts) return EKV_OK;
+  // a block's own prefix sums cost about as much as a few thousand slots
+  const int64_t fresh = (int64_t)batch * width < n_free ? (int64_t)batch * width : n_free;    // at most
+  int64_t most = (int64_t)n_slots > batch ? n_slots : batch;
+  if (fresh / 8 > most) most = fresh / 8;
+  int64_t blocks = (most + 4 * kPlanThreads - 1) / (4 * kPlanThreads);
+  if (blocks > 2 * sm_count()) blocks = 2 * sm_count();
+  return plan_launch<false>(a, (int)(blocks > 0 ? blocks : 1), stream);
+}
+
+extern "C" int ekv_release_blocks(const int32_t* seq_lens, const int32_t* keep_lens, int32_t keep_all, int32_t batch,
+                                  int32_t page_size, int32_t* block_table, int64_t bt_stride, int32_t width,
+                                  int32_t* free_blocks, int32_t n_free, int32_t* status, void* stream) {
+  using namespace ekv;
+  PlanArgs a{seq_lens, keep_lens, keep_all, batch, page_size, block_table, bt_stride, width, free_blocks, n_free,
+             nullptr, nullptr, 0, nullptr, status};
+  if (int e = plan_check(a)) return e;
+  if (batch == 0) return EKV_OK;
+  const int64_t most = (int64_t)batch * (width > 0 ? width : 1);
+  int64_t blocks = (most + 16 * kPlanThreads - 1) / (16 * kPlanThreads);
+  if (blocks > sm_count()) blocks = sm_count();
+  return plan_launch<true>(a, (int)blocks, stream);
+}

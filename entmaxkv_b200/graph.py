@@ -158,8 +158,7 @@ class DecodeStepGraph:
         valid once the current stream has been synchronised."""
         cache = self.cache
         io = self.pinned_io()
-        if cache.seq_len + 1 > cache.capacity:
-            cache.reserve(max(cache.capacity + 4096, cache.capacity * 5 // 4))
+        cache._make_room([n + 1 for n in cache._host_lens])
         if self.graph_io is None or self._captured_capacity_io != cache.capacity:
             self.q.copy_(io["q"], non_blocking=True)      # the capture's eager warm-up pass runs on the real query
             self._capture(with_io=True)
@@ -169,8 +168,7 @@ class DecodeStepGraph:
 
     def step(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> torch.Tensor:
         cache = self.cache
-        if cache.seq_len + 1 > cache.capacity:
-            cache.reserve(max(cache.capacity + 4096, cache.capacity * 5 // 4))
+        cache._make_room([n + 1 for n in cache._host_lens])
         # inputs first: the eager warm-up pass of a (re)capture then runs on this step's real query
         # (an all-zero query would make every page pass the Gaussian threshold)
         stage_inputs(((self.q, q), (self.k_new, k_new), (self.v_new, v_new)))

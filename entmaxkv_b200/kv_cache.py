@@ -18,6 +18,9 @@ Differences a user can observe:
     table, the layout serving engines hand out (the reference cache is dense,
     kv_cache.py:44-56).  Pages of one sequence are then not contiguous in memory; the page
     statistics stay dense.  ``k_cache`` / ``v_cache`` are gathered copies in that mode.
+  * with ``num_blocks`` that pool is shared: pages get their blocks when tokens arrive (planned on the GPU from the
+    lengths, no host synchronisation) and ``release`` gives them back.
+  * ``extend`` writes several tokens per sequence: a prompt chunk, or the accepted path of a tree of drafted tokens.
 """
 
 from __future__ import annotations
@@ -37,22 +40,29 @@ class PagedKVCache:
     DEFAULT_HEADROOM = 1024
 
     def __init__(self, page_size: int = 16, capacity: Optional[int] = None, block_table: bool = False,
-                 block_order: str = "interleaved"):
+                 block_order: str = "interleaved", num_blocks: Optional[int] = None):
         if page_size <= 0:
             raise ValueError("page_size must be positive")
         if block_order not in ("interleaved", "random"):
             raise ValueError("block_order must be 'interleaved' or 'random'")
+        if num_blocks is not None and (not block_table or num_blocks <= 0):
+            raise ValueError("num_blocks must be positive and needs block_table=True")
         self.page_size = int(page_size)
         self._requested_capacity = capacity
         #: K/V live in a pool of physical blocks behind a block table (see the module docstring)
         self.block_mode = bool(block_table)
         self._block_order = block_order
+        #: blocks of the shared pool; None: every sequence owns page_capacity blocks from the start
+        self.num_blocks = num_blocks
+        self._free = None                      # int32 [num_blocks]: the shared pool as a stack (block_tables.py)
         self._table = None                     # int32 [B, page_capacity]: page -> physical block
         self._pool_k = self._pool_v = None     # [num_blocks, H_kv, page_size, D]
         self._k = self._v = None
         self._meta = None                      # [4, B, H, page_capacity, D]: min, max, mean, std
         self.seq_lens: Optional[torch.Tensor] = None     # int32 [B] on the device
         self._host_lens: list[int] = []
+        self._lens_exact = True                # False: device lengths may be below the host's
+        self._may_be_empty = False             # True: a sequence may hold no token (released, or rewound to 0)
         self._ctl = None                       # int32: [0]=status, [16:16+B] append tickets
         self.last_num_selected_per_head = None
         self._scratch: dict = {}
@@ -128,6 +138,9 @@ class PagedKVCache:
     def _allocate(self, B, H, D, capacity, dtype, device):
         P = self.page_size
         capacity = (capacity + P - 1) // P * P
+        if self.num_blocks is not None:
+            self._allocate_shared(B, H, D, capacity, dtype, device)
+            return
         self._k = torch.empty(B, H, capacity, D, dtype=dtype, device=device)
         self._v = torch.empty(B, H, capacity, D, dtype=dtype, device=device)
         self._meta = torch.zeros(4, B, H, capacity // P, D, dtype=dtype, device=device)
@@ -153,6 +166,25 @@ class PagedKVCache:
                 table[:, pcap_old:] = fresh.view(B, pcap - pcap_old)
             self._table = table
 
+    def _allocate_shared(self, B, H, D, capacity, dtype, device):
+        """Shared pool: [num_blocks, H, P, D] behind an empty table; ``capacity`` only bounds a sequence's pages."""
+        P, old = self.page_size, self._table
+        if old is None:
+            self._pool_k = torch.empty(self.num_blocks, H, P, D, dtype=dtype, device=device)
+            self._pool_v = torch.empty_like(self._pool_k)
+            self._free = torch.arange(self.num_blocks, dtype=torch.int32, device=device)
+            if self._block_order == "random":
+                g = torch.Generator(device="cpu").manual_seed(1234)
+                self._free = torch.randperm(self.num_blocks, generator=g).to(torch.int32).to(device)
+        # only the SHAPE of the dense cache (the wrappers read sizes from it); the rows live in the pool
+        self._k = self._pool_k.new_empty(1).expand(B, H, capacity, D)
+        self._v = self._k
+        self._meta = torch.zeros(4, B, H, capacity // P, D, dtype=dtype, device=device)
+        self._table = torch.full((B, capacity // P), -1, dtype=torch.int32, device=device)
+        if old is not None:
+            self._table[:, :old.shape[1]] = old
+        self._desc = None
+
     def initialize(self, k: torch.Tensor, v: torch.Tensor,
                    seq_lens: Optional[Sequence[int]] = None, capacity: Optional[int] = None):
         """Copy prefill keys/values in and build every page's statistics in one launch.
@@ -171,14 +203,20 @@ class PagedKVCache:
         cap = capacity or self._requested_capacity or (S + self.DEFAULT_HEADROOM)
         if cap < S:
             raise ValueError("capacity is smaller than the prefill length")
+        if self.num_blocks is not None and sum(-(-n // self.page_size) for n in lens) > self.num_blocks:
+            raise RuntimeError(f"the prefill does not fit the pool of {self.num_blocks} blocks")
         self._table = None
         self._allocate(B, H, D, cap, k.dtype, k.device)
+        if self.num_blocks is not None:
+            self._plan(torch.zeros(B, dtype=torch.int32, device=k.device),
+                       torch.tensor(lens, dtype=torch.int32, device=k.device))
         if self.block_mode:
-            self._scatter_pages(k, v)
+            self._scatter_pages(k, v, lens)
         else:
             self._k[:, :, :S].copy_(k)
             self._v[:, :, :S].copy_(v)
         self._host_lens = lens
+        self._lens_exact, self._may_be_empty = True, False
         self.seq_lens = torch.tensor(lens, dtype=torch.int32, device=k.device)
         self._ctl = torch.zeros(16 + B, dtype=torch.int32, device=k.device)
         self._scratch = {}
@@ -186,16 +224,26 @@ class PagedKVCache:
         _lib.check(lib.ekv_page_stats_init(C.byref(self.desc()), max(lens), _lib.stream_ptr()),
                    "ekv_page_stats_init")
 
-    def _scatter_pages(self, k, v):
+    def _plan(self, seq_lens, new_lens, status=None):
+        """Shared pool: blocks for the pages that ``new_lens`` more tokens need."""
+        from .block_tables import plan_block_tables
+        plan_block_tables(seq_lens, new_lens, self._table, self._free, self.page_size, status=status)
+
+    def _scatter_pages(self, k, v, lens):
         """Block mode: copy [B, H, S, D] tensors page by page into the blocks the table assigns."""
         B, H, S, D = k.shape
         P = self.page_size
         n = (S + P - 1) // P
         ids = self._table[:, :n].reshape(-1).long()
+        held = None
+        if self.num_blocks is not None:        # pages behind a short sequence have no block
+            held = torch.tensor([p * P < m for m in lens for p in range(n)], device=ids.device)
+            ids = ids[held]
         for src, pool in ((k, self._pool_k), (v, self._pool_v)):
             if n * P != S:
                 src = torch.cat([src, src.new_zeros(B, H, n * P - S, D)], dim=2)
-            pool[ids] = src.view(B, H, n, P, D).permute(0, 2, 1, 3, 4).reshape(B * n, H, P, D)
+            pages = src.reshape(B, H, n, P, D).permute(0, 2, 1, 3, 4).reshape(B * n, H, P, D)
+            pool[ids] = pages if held is None else pages[held]
 
     def translate(self, page_indices: torch.Tensor, counts: torch.Tensor, out: Optional[torch.Tensor] = None):
         """Block mode: page numbers -> physical block ids for the first ``counts[b, h]`` entries of every
@@ -219,7 +267,9 @@ class PagedKVCache:
         old_k, old_v, old_meta, S = self._k, self._v, self._meta, self.seq_len
         old_pools = (self._pool_k, self._pool_v)
         self._allocate(B, H, D, capacity, old_k.dtype, old_k.device)
-        if self.block_mode:
+        if self.num_blocks is not None:
+            pass                               # the pool stays, only the table and the statistics got wider
+        elif self.block_mode:
             if self._block_order == "interleaved":
                 # block ids p*B + b do not depend on the capacity: the old blocks keep their numbers
                 n_old = old_pools[0].shape[0]
@@ -247,14 +297,140 @@ class PagedKVCache:
             raise ValueError("k_new / v_new dtype differs from the cache dtype")
         if k_new.stride(-1) != 1 or v_new.stride(-1) != 1 or k_new.stride() != v_new.stride():
             k_new, v_new = k_new.contiguous(), v_new.contiguous()
-        if self.seq_len + 1 > self.capacity:
-            self.reserve(max(self.capacity + 4096, self.capacity * 5 // 4))
+        if self.num_blocks is not None:        # a new page needs its block first
+            self.extend(k_new, v_new)
+            return
+        self._make_room([n + 1 for n in self._host_lens])
         lib = _lib.load()
         _lib.check(lib.ekv_append(C.byref(self.desc()), k_new.data_ptr(), v_new.data_ptr(),
                                   k_new.stride(0), k_new.stride(1),
                                   self._ctl[16:].data_ptr(), self._ctl.data_ptr(), _lib.stream_ptr()),
                    "ekv_append")
         self._host_lens = [n + 1 for n in self._host_lens]
+        self._may_be_empty = False
+
+    def extend(self, k_new: torch.Tensor, v_new: torch.Tensor, counts=None, index: Optional[torch.Tensor] = None,
+               start=None, max_seq_len: Optional[int] = None):
+        """Append several tokens per sequence and refresh the statistics of every page that they touch.
+
+        k_new, v_new: [B, H_kv, T, D], any strides.  ``counts`` ([B]): how many rows each sequence gets (default T);
+        ``index`` (int32 CUDA [B, T]): which row goes where (row ``index[b, i]`` at the i-th new position: the accepted
+        path of a tree of drafted tokens; default: row i).  ``start`` ([B]): the first position to write, at most the
+        current length: a smaller one rewinds the sequence, whose length becomes ``start + counts``.
+
+        ``counts`` and ``start`` are sequences of ints, or int32 CUDA tensors.  The host does not read the latter, so
+        its view of the lengths (``seq_len``, ``host_seq_lens``, the row range of ``k_cache``) becomes an upper bound:
+        ``T`` more tokens for every sequence, or ``max_seq_len`` where that is given and smaller (rows past it are then
+        the caller's mistake).  ``sync_lengths`` makes it exact again.  Values out of range are clipped on the device and
+        show in ``device_status``.
+        """
+        if self._k is None:
+            raise RuntimeError("initialize() the cache before extend()")
+        _lib.require_cuda(k_new, v_new)
+        B, H, _, D = self._k.shape
+        if k_new.dim() != 4 or k_new.shape != v_new.shape or (k_new.shape[0], k_new.shape[1], k_new.shape[3]) != (B, H, D):
+            raise ValueError(f"k_new / v_new must be [{B}, {H}, T, {D}]")
+        if k_new.dtype != self._k.dtype or v_new.dtype != self._k.dtype:
+            raise ValueError("k_new / v_new dtype differs from the cache dtype")
+        device, T = self._k.device, k_new.shape[2]
+        _lib.require_same_device(device, k_new, v_new, index)
+        if max_seq_len is not None and max_seq_len < 0:
+            raise ValueError("max_seq_len must be >= 0")
+        if index is not None and (index.dtype != torch.int32 or tuple(index.shape) != (B, T)
+                                  or (T > 1 and index.stride(1) != 1)):
+            raise ValueError(f"index must be int32 [{B}, {T}], contiguous along the tokens")
+        counts_host, counts = self._row_lens(counts, "counts", T)
+        start_host, start = self._row_lens(start, "start", None)
+        bound = [min(s, n) if start_host is not None else n for s, n in zip(start_host or self._host_lens, self._host_lens)]
+        bound = [n + m for n, m in zip(bound, counts_host or [T] * B)]
+        if max_seq_len is not None:
+            bound = [min(n, max_seq_len) for n in bound]
+        rewound_on_device = start is not None and start_host is None
+        if T == 0:
+            if start is None:
+                return
+            k_new = v_new = k_new.new_zeros(B, H, 1, D)      # a rewind alone: no row is taken
+            counts, T, index = torch.zeros(B, dtype=torch.int32, device=device), 1, None
+        e = k_new.element_size()
+        s = k_new.stride()
+        if (s != v_new.stride() or s[3] != 1 or s[0] * e % 16 or s[1] * e % 16 or s[2] * e % 16
+                or (k_new.data_ptr() | v_new.data_ptr()) % 16):
+            k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
+            s = k_new.stride()
+        with _lib.on_device(k_new):
+            self._make_room(bound)
+            if self.num_blocks is not None:
+                held = self.seq_lens
+                if start is not None:          # what lies behind the rewind goes back first
+                    from .block_tables import return_blocks
+                    return_blocks(held, start, self._table, self._free, self.page_size, status=self._ctl)
+                    held = torch.minimum(held, start.clamp(min=0))
+                self._plan(held, T if counts is None else counts, status=self._ctl)
+            _lib.check(_lib.load().ekv_extend(
+                C.byref(self.desc()), k_new.data_ptr(), v_new.data_ptr(), s[0], s[1], s[2], T, _lib.ptr(counts),
+                _lib.ptr(index), index.stride(0) if index is not None and B > 1 else T, _lib.ptr(start),
+                self._ctl[16:].data_ptr(), self._ctl.data_ptr(), _lib.stream_ptr()), "ekv_extend")
+        if counts_host is None or rewound_on_device:
+            self._lens_exact = False
+        if counts_host is not None and min(counts_host) > 0:
+            self._may_be_empty = False
+        elif rewound_on_device or (start_host is not None and 0 in start_host):
+            self._may_be_empty = True
+        self._host_lens = bound
+
+    def _make_room(self, lens):
+        """Before tokens are added: room for sequences of ``lens`` tokens (upper bounds), and blocks in a shared pool."""
+        if max(lens) > self.capacity:
+            self.reserve(max(max(lens), self.capacity + 4096, self.capacity * 5 // 4))
+        if self.num_blocks is not None and sum(-(-n // self.page_size) for n in lens) > self.num_blocks:
+            raise RuntimeError(f"the pool of {self.num_blocks} blocks may not suffice: release() sequences" + (
+                "" if self._lens_exact else ", or call sync_lengths() (the host knows only upper bounds of the lengths)"))
+
+    def _row_lens(self, value, name, most):
+        """One length per sequence, given on the host or on the device: (host list or None, int32 CUDA tensor or None)."""
+        B, device = self._k.shape[0], self._k.device
+        if value is None:
+            return ([most] * B if most is not None else None), None
+        if isinstance(value, torch.Tensor):
+            _lib.require_cuda(value)
+            _lib.require_same_device(device, value)
+            if value.dtype != torch.int32 or tuple(value.shape) != (B,) or not value.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 [{B}] tensor")
+            return None, value
+        host = [int(x) for x in value]
+        if len(host) != B or min(host) < 0 or (most is not None and max(host) > most):
+            raise ValueError(f"{name} must hold one length per sequence" + (f", at most {most}" if most is not None else ""))
+        if most is None and self._lens_exact and any(s > n for s, n in zip(host, self._host_lens)):
+            raise ValueError(f"{name} lies beyond the sequence's length")
+        return host, torch.tensor(host, dtype=torch.int32, device=device)
+
+    def sync_lengths(self) -> list[int]:
+        """Read the sequence lengths back from the device (synchronises): after ``extend`` with lengths on the device the
+        host's view is an upper bound."""
+        self._host_lens = self.seq_lens.tolist()
+        self._lens_exact, self._may_be_empty = True, min(self._host_lens) < 1
+        return list(self._host_lens)
+
+    def release(self, rows: Sequence[int]):
+        """Empty the sequences ``rows``; with a shared pool their blocks go back to it.  A released sequence takes new
+        tokens through ``extend`` and can be attended to once it has some."""
+        if self._k is None:
+            raise RuntimeError("initialize() the cache before release()")
+        B = self._k.shape[0]
+        rows = sorted({int(r) for r in rows})
+        if rows and not 0 <= rows[0] <= rows[-1] < B:
+            raise ValueError(f"rows must lie in [0, {B})")
+        if not rows:
+            return
+        keep = self.seq_lens.clone()
+        keep[torch.tensor(rows, device=keep.device)] = 0
+        if self.num_blocks is not None:
+            from .block_tables import release_block_tables
+            release_block_tables(self.seq_lens, keep, self._table, self._free, self.page_size, status=self._ctl)
+        else:
+            self.seq_lens.copy_(keep)
+        self._host_lens = [0 if i in rows else n for i, n in enumerate(self._host_lens)]
+        self._may_be_empty = True
 
     # ------------------------------------------------------------------ C ABI view
 
@@ -263,7 +439,8 @@ class PagedKVCache:
         if self._desc is None:
             k, m = self._k, self._meta
             d = _lib.CacheDesc()
-            d.k, d.v = k.data_ptr(), self._v.data_ptr()
+            kp, vp = (k, self._v) if self.num_blocks is None else (self._pool_k, self._pool_v)
+            d.k, d.v = kp.data_ptr(), vp.data_ptr()
             d.k_min, d.k_max, d.k_mean, d.k_std = (m[i].data_ptr() for i in range(4))
             d.kv_stride_b, d.kv_stride_h = k.stride(0), k.stride(1)
             d.meta_stride_b, d.meta_stride_h = m.stride(1), m.stride(2)

@@ -1,0 +1,87 @@
+"""RMS norm of every query and key head together with the position rotation.
+
+What lies between a layer's projection and ``PagedKVCache.append`` / ``extend``: the reference leaves it to the model
+around it (its decode takes rotated keys, entmaxkv/kv_cache.py:72).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+_STRIDES = C.c_int64 * 3
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself when its rows are 16-byte aligned and contiguous, else a copy."""
+    e = t.element_size()
+    s = t.stride()
+    if s[3] != 1 or t.data_ptr() % 16 or s[0] * e % 16 or s[1] * e % 16 or s[2] * e % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _destination(out, like, name):
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{name} must match its input in shape, dtype and device")
+    if out.numel() and (_rows(out) is not out or any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride()))):
+        raise ValueError(f"{name} must have contiguous, 16-byte aligned rows of its own")
+    return out
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 eps: Optional[float] = 1e-6, interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None):
+    """Norm and rotate the queries [B, H_q, T, D] and keys [B, H_kv, T, D] of T tokens per sequence.
+
+    ``y = x * rsqrt(mean(x^2) + eps) * weight`` over each head vector (``eps=None``: no norm, and no weights), then the
+    first ``2 * len(inv_freq)`` elements of y are rotated by ``position * inv_freq[j]``: the pairs are (j, j + half), or
+    (2j, 2j + 1) with ``interleaved``.  Computed in fp32 (the angle in 64 bits) and rounded once.  q and k may be views
+    of a fused projection (any strides).  ``positions``: int32 or int64, [B, T] or [T]; ``inv_freq``: fp32, a multiple
+    of 8 entries, at most D / 2; weights: [D], both in the tensors' dtype or both fp32.  ``q_out`` / ``k_out`` may be
+    the inputs themselves (in place) and must not overlap them otherwise.  Returns (q_out, k_out).
+    """
+    _lib.require_cuda(q, k, positions, inv_freq, q_weight, k_weight)
+    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+        raise ValueError("q must be [B, H_q, T, D] and k [B, H_kv, T, D]")
+    B, Hq, T, D = q.shape
+    if q.dtype != k.dtype:
+        raise ValueError("q and k must have one dtype")
+    code = _lib.dtype_code(q.dtype)
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((B, T), (T,)):
+        raise ValueError(f"positions must be int32 or int64, [{B}, {T}] or [{T}]")
+    half = inv_freq.shape[0] if inv_freq.dim() == 1 else -1
+    if half < 0 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or half % 8 or 2 * half > D:
+        raise ValueError("inv_freq must be contiguous fp32 with a multiple of 8 entries, at most head_dim / 2")
+    weight_f32 = 0
+    if q_weight is not None or k_weight is not None:
+        if eps is None:
+            raise ValueError("weights belong to the norm; eps=None switches it off")
+        for w in (q_weight, k_weight):
+            if w is not None and (tuple(w.shape) != (D,) or w.dtype not in (q.dtype, torch.float32)
+                                  or not w.is_contiguous()):
+                raise ValueError(f"weights must be contiguous [{D}] tensors in the dtype of q or fp32")
+        if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+            raise ValueError("q_weight and k_weight must have one dtype")
+        weight_f32 = int((k_weight if q_weight is None else q_weight).dtype == torch.float32)
+    if eps is not None and not eps >= 0:
+        raise ValueError("eps must be >= 0 (or None)")
+    _lib.require_same_device(q.device, k, positions, inv_freq, q_weight, k_weight)
+    with _lib.on_device(q):
+        q_out, k_out = _destination(q_out, q, "q_out"), _destination(k_out, k, "k_out")
+        q, k = _rows(q), _rows(k)
+        _lib.check(_lib.load().ekv_qk_norm_rope(
+            code, B, T, Hq, k.shape[1], D, q.data_ptr(), _STRIDES(*q.stride()[:3]), k.data_ptr(),
+            _STRIDES(*k.stride()[:3]), q_out.data_ptr(), _STRIDES(*q_out.stride()[:3]), k_out.data_ptr(),
+            _STRIDES(*k_out.stride()[:3]), positions.data_ptr(), int(positions.dtype == torch.int64),
+            positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1), inv_freq.data_ptr(), half,
+            int(interleaved), _lib.ptr(q_weight), _lib.ptr(k_weight), weight_f32, int(eps is not None),
+            0.0 if eps is None else eps, _lib.stream_ptr()), "ekv_qk_norm_rope")
+    return q_out, k_out

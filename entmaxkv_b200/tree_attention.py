@@ -1,0 +1,84 @@
+"""Entmax attention of a tree of drafted tokens over the cache (speculative decoding).
+
+The reference decodes one token per sequence and step (entmaxkv/attention_topk.py:8-100); a step that verifies several
+drafted tokens at once attends with all of them, each seeing the cache and its own ancestors in the tree.  The drafted
+keys and values stay outside the cache; ``PagedKVCache.extend`` writes the accepted ones.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .kv_cache import PagedKVCache
+from .rope import _STRIDES, _rows
+
+#: drafted tokens per sequence
+MAX_TOKENS = 256
+
+
+def tree_attention_decode(q: torch.Tensor, kv_cache: PagedKVCache, k_draft: torch.Tensor, v_draft: torch.Tensor,
+                          tree_mask: torch.Tensor, out: torch.Tensor, draft_lens: Optional[torch.Tensor] = None,
+                          alpha: float = 1.5, taus_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attend with T drafted tokens per sequence to the whole cache and to each token's part of the tree.
+
+    q, out [B, H_q, T, D]; k_draft, v_draft [B, H_kv, T, D] in the cache's dtype (any strides).  ``tree_mask``: bool,
+    [T, T] or [B, T, T]: token t sees drafted token j where ``tree_mask[..., t, j]`` (itself included only where it says
+    so), and every token of the cache.  ``draft_lens`` (int32 CUDA [B]): trees of different sizes; tokens from there on
+    are neither keys nor rows, and their rows of ``out`` and ``taus_out`` stay as they were.
+
+    ``p = ((alpha-1) q.k / sqrt(D) - tau)_+^(1/(alpha-1))`` with the tau that makes each row sum to one, solved until it
+    no longer moves; ``out = sum p v``, written in place and returned.  A row that sees nothing gets zeros and
+    ``tau = +inf``; a NaN or infinite score makes its row NaN.  ``taus_out`` (fp32 [B, H_q, T], contiguous) receives the
+    thresholds.  Works on dense and block-table caches; the cache is not changed.
+    """
+    if kv_cache._k is None:
+        raise RuntimeError("kv_cache is not initialised")
+    if not alpha > 1.0:
+        raise ValueError("alpha must be > 1")
+    _lib.require_cuda(q, k_draft, v_draft, tree_mask, out, draft_lens, taus_out)
+    B, Hkv, _, D = kv_cache._k.shape
+    dtype, device = kv_cache._k.dtype, kv_cache._k.device
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[1] == 0 or q.shape[1] % Hkv:
+        raise ValueError(f"q must be [{B}, H_q, T, {D}] with H_q a multiple of {Hkv}")
+    Hq, T = q.shape[1], q.shape[2]
+    if T > MAX_TOKENS:
+        raise ValueError(f"at most {MAX_TOKENS} drafted tokens per sequence")
+    if tuple(k_draft.shape) != (B, Hkv, T, D) or tuple(v_draft.shape) != (B, Hkv, T, D):
+        raise ValueError(f"k_draft / v_draft must be [{B}, {Hkv}, {T}, {D}]")
+    if q.dtype != dtype or k_draft.dtype != dtype or v_draft.dtype != dtype or out.dtype != dtype:
+        raise ValueError("q, k_draft, v_draft and out must have the cache's dtype")
+    if out.shape != q.shape or (T and out.stride(-1) != 1) or any(
+            n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError("out must match q in shape and be contiguous along head_dim")
+    if tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((T, T), (B, T, T)) or (
+            T > 1 and tree_mask.stride(-1) != 1):
+        raise ValueError(f"tree_mask must be bool [{T}, {T}] or [{B}, {T}, {T}], contiguous along its last axis")
+    if draft_lens is not None and (draft_lens.dtype != torch.int32 or tuple(draft_lens.shape) != (B,)
+                                   or not draft_lens.is_contiguous()):
+        raise ValueError(f"draft_lens must be a contiguous int32 [{B}] tensor")
+    if taus_out is not None and (tuple(taus_out.shape) != (B, Hq, T) or taus_out.dtype != torch.float32
+                                 or not taus_out.is_contiguous()):
+        raise ValueError("taus_out must be a contiguous fp32 [B, H_q, T] tensor")
+    _lib.require_same_device(device, q, k_draft, v_draft, tree_mask, out, draft_lens, taus_out)
+    if T == 0:
+        return out
+    with _lib.on_device(q):
+        lib = _lib.load()
+        q, k_draft, v_draft = _rows(q), _rows(k_draft), _rows(v_draft)
+        # a captured call is replayed while the sequences grow: it is sized by the capacity
+        capturing = torch.cuda.is_current_stream_capturing()
+        bound = kv_cache.capacity if capturing else min(kv_cache.seq_len, kv_cache.capacity)
+        desc = C.byref(kv_cache.desc())
+        # scratch of this call alone, from torch's stream-ordered allocator: two streams or two graphs never share it
+        ws = torch.empty(lib.ekv_tree_workspace_bytes(desc, Hq, T, bound), dtype=torch.uint8, device=device)
+        _lib.check(lib.ekv_tree_decode(
+            desc, q.data_ptr(), _STRIDES(*q.stride()[:3]), Hq, T, k_draft.data_ptr(), _STRIDES(*k_draft.stride()[:3]),
+            v_draft.data_ptr(), _STRIDES(*v_draft.stride()[:3]), tree_mask.data_ptr(),
+            tree_mask.stride(0) if tree_mask.dim() == 3 else 0, tree_mask.stride(-2), _lib.ptr(draft_lens), bound,
+            float(alpha), out.data_ptr(), _STRIDES(*out.stride()[:3]), _lib.ptr(taus_out), ws.data_ptr(), ws.numel(),
+            kv_cache._ctl.data_ptr(), _lib.stream_ptr()), "ekv_tree_decode")
+    return out

@@ -120,6 +120,62 @@ int ekv_append(const ekv_cache_desc* c, const void* k_new, const void* v_new,
 int ekv_append_static(const ekv_cache_desc* c, const void* k_new, const void* v_new,
                       int64_t new_stride_b, int64_t new_stride_h, int32_t* status, void* stream);
 
+/* Several tokens per sequence in one call (a prompt chunk, or the accepted path of a tree of drafted
+ * tokens): for i < counts[b], row index[b, i] (null: row i) of k_new / v_new [B, H_kv, tokens, D] is
+ * written at position start[b] + i, the statistics of every page touched are refreshed and seq_lens[b]
+ * becomes start[b] + counts[b].  start null: the current lengths; a start below the current length rewinds
+ * the sequence.  counts null: all `tokens`.  Device values out of range (counts beyond `tokens`, a start
+ * beyond the length, an index outside the rows) are clipped and set EKV_STATUS_TOKENS, rows past the
+ * capacity or past the last page that has a block are dropped and set EKV_STATUS_CAPACITY /
+ * EKV_STATUS_PAGE_RANGE.  counters as ekv_append.  No counterpart in the reference, whose append takes one
+ * token (entmaxkv/kv_cache.py:72-116); the statistics are those of ekv_page_stats_init. */
+int ekv_extend(const ekv_cache_desc* c, const void* k_new, const void* v_new, int64_t new_stride_b,
+               int64_t new_stride_h, int64_t new_stride_t, int32_t tokens, const int32_t* counts,
+               const int32_t* index, int64_t index_stride_b, const int32_t* start, int32_t* counters,
+               int32_t* status, void* stream);
+
+/* ---- block tables and slot maps ------------------------------------------ */
+
+#define EKV_PLAN_MAX_BATCH 16384
+
+/* Pages and slots for new_lens[b] (null: new_all) more tokens of every sequence.  With held[b] =
+ * ceil(seq_lens[b] / page_size) and need[b] = ceil((seq_lens[b] + new_lens[b]) / page_size), page p in
+ * [held[b], need[b]) gets block_table[b, p] = free_blocks[sum(held) + sum_{b' < b}(need - held) + p - held[b]],
+ * or -1 past the end of the list.  The list is a stack whose lowest sum(held) places are in use: their
+ * content does not matter, and the call changes nothing but table entries behind a sequence's held pages,
+ * so it can be repeated.  The new tokens of all sequences, one after another, get
+ *   slots[r] = block * page_size + position % page_size (-1 without a block), positions[r] = position,
+ * both -1 from the last token on; row_starts[b] (B + 1 entries) is where sequence b's tokens begin.
+ * slots, positions, row_starts and status may be null; status gets EKV_STATUS_CAPACITY when the pool or the
+ * table's width does not suffice.  batch <= EKV_PLAN_MAX_BATCH. */
+int ekv_plan_block_tables(const int32_t* seq_lens, const int32_t* new_lens, int32_t new_all, int32_t batch,
+                          int32_t page_size, int32_t* block_table, int64_t bt_stride, int32_t width,
+                          const int32_t* free_blocks, int32_t n_free, int64_t* slots, int32_t* positions,
+                          int32_t n_slots, int32_t* row_starts, int32_t* status, void* stream);
+
+/* The way back: the pages of every sequence behind its first keep_lens[b] (null: keep_all) tokens return to
+ * the list, in sequence order on top of what stays in use, and their table entries become -1.  seq_lens is
+ * only read: the caller lowers it to keep_lens afterwards. */
+int ekv_release_blocks(const int32_t* seq_lens, const int32_t* keep_lens, int32_t keep_all, int32_t batch,
+                       int32_t page_size, int32_t* block_table, int64_t bt_stride, int32_t width,
+                       int32_t* free_blocks, int32_t n_free, int32_t* status, void* stream);
+
+/* ---- norm and rotation of queries and keys --------------------------------- */
+
+/* y = x * rsqrt(mean(x^2) + eps) * weight per head vector (norm != 0), then the first 2 * half elements are
+ * rotated by position * inv_freq[j]: pairs (j, j + half), or (2j, 2j + 1) when interleaved.  fp32 throughout
+ * (the angle in 64 bits), one rounding.  x: q [B, H_q, tokens, D] and k [B, H_kv, tokens, D] with element
+ * strides {batch, head, token}; an output may be its input.  positions: int32 or (positions_64) int64 with
+ * the given strides; inv_freq fp32 [half], half a multiple of 8; weights [D] in x's dtype or (weight_f32)
+ * fp32, null: 1.  kv_heads may be 0. */
+int ekv_qk_norm_rope(int32_t dtype, int32_t batch, int32_t tokens, int32_t q_heads, int32_t kv_heads,
+                     int32_t head_dim, const void* q, const int64_t* q_strides, const void* k,
+                     const int64_t* k_strides, void* q_out, const int64_t* q_out_strides, void* k_out,
+                     const int64_t* k_out_strides, const void* positions, int32_t positions_64,
+                     int64_t pos_stride_b, int64_t pos_stride_t, const float* inv_freq, int32_t half,
+                     int32_t interleaved, const void* q_weight, const void* k_weight, int32_t weight_f32,
+                     int32_t norm, float eps, void* stream);
+
 /* ---- top-k page selection ---------------------------------------------- */
 
 /* score[b,h,p] = sum_d max(q_d*kmin[p,d], q_d*kmax[p,d]) for every page but the
@@ -257,6 +313,29 @@ int ekv_gaussian_select(const ekv_cache_desc* c, int32_t q_heads, int32_t max_se
 int ekv_tau_clamp(const float* tau_hat, int64_t tau_hat_stride, const float* cap_max,
                   const float* tau_floor, int32_t n, float alpha, float eps, float* tau,
                   void* stream);
+
+/* ---- a tree of drafted tokens ---------------------------------------------- */
+
+#define EKV_TREE_MAX_TOKENS 256
+
+/* Entmax attention of `tokens` drafted tokens per sequence (speculative decoding): row (b, h, t) of q
+ * [B, H_q, tokens, D] sees every token of the cache's sequence b and the drafted tokens j < draft_lens[b]
+ * (null: all) with mask[b, t, j] != 0 (bytes; mask_stride_b 0 for one mask), whose keys and values are
+ * k_draft / v_draft [B, H_kv, tokens, D].  z = (alpha-1)/sqrt(D) q.k; tau is the converged root of
+ * sum (z - tau)_+^(1/(alpha-1)) = 1 and out = sum (z - tau)_+^(1/(alpha-1)) v.  A row that sees nothing gets
+ * zeros and tau = +inf, one with a NaN or +inf score NaN; rows t >= draft_lens[b] of out and tau stay as
+ * they were.  The cache is only read.  Strides {batch, head, token} in elements; tau [B, H_q, tokens]
+ * contiguous, may be null.  max_seq_len: host-side upper bound of seq_lens[], at most the capacity (longer
+ * sequences are cut to it).  The workspace needs no initialisation; its size grows with rows * max_seq_len
+ * up to about 2 GiB, then the (sequence, KV head) groups are taken in several turns.
+ * The reference decodes one token at a time (entmaxkv/attention_topk.py:8-100). */
+size_t ekv_tree_workspace_bytes(const ekv_cache_desc* c, int32_t q_heads, int32_t tokens, int32_t max_seq_len);
+int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int64_t* q_strides, int32_t q_heads,
+                    int32_t tokens, const void* k_draft, const int64_t* k_strides, const void* v_draft,
+                    const int64_t* v_strides, const uint8_t* mask, int64_t mask_stride_b, int64_t mask_stride_t,
+                    const int32_t* draft_lens, int32_t max_seq_len, float alpha, void* out,
+                    const int64_t* out_strides, float* tau, void* workspace, size_t workspace_bytes,
+                    int32_t* status, void* stream);
 
 /* ---- paged entmax decode ------------------------------------------------ */
 
