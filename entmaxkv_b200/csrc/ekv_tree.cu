@@ -1,5 +1,5 @@
 // Entmax attention of a tree of drafted tokens over the cache (see ekv_tree.cuh for the method).
-#include "ekv_tree.cuh"
+#include "ekv_tree_mma.cuh"
 
 namespace ekv {
 
@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
       const int64_t at = row_id * a.max_parts * a.sub + part * a.sub + warp;
       a.counts[at] = count;
       a.maxima[at] = top;
+      a.bounds[at] = top - 1.f;
     }
   }
 }
@@ -218,16 +219,27 @@ __global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_c
   const int lists = parts * a.sub;
   const int* const counts = a.counts + row_id * a.max_parts * a.sub;
   const float* const maxima = a.maxima + row_id * a.max_parts * a.sub;
-  float top = -INFINITY;
+  const float* const bounds = a.bounds + row_id * a.max_parts * a.sub;
+  float top = -INFINITY, floor_z = -INFINITY;
   __syncthreads();                               // s_zd
-  for (int i = tid; i < lists; i += kFinThreads) top = max_nan(top, maxima[i]);
+  for (int i = tid; i < lists; i += kFinThreads) {
+    top = max_nan(top, maxima[i]);
+    floor_z = fmaxf(floor_z, bounds[i]);
+  }
   for (int j = tid; j < a.tokens; j += kFinThreads) top = max_nan(top, s_zd[j]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) scratch[warp] = top;
+  floor_z = warp_max(floor_z);
+  if (lane == 0) {
+    scratch[warp] = top;
+    scratch[8 + warp] = floor_z;
+  }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kFinThreads / 32; ++w) top = max_nan(top, scratch[w]);
+  for (int w = 0; w < kFinThreads / 32; ++w) {
+    top = max_nan(top, scratch[w]);
+    floor_z = fmaxf(floor_z, scratch[8 + w]);
+  }
 
   T* const out = static_cast<T*>(a.out) + b * a.os[0] + hq * a.os[1] + t * a.os[2];
   float* const tau_out = a.tau ? a.tau + ((int64_t)b * a.q_heads + hq) * a.tokens + t : nullptr;
@@ -237,7 +249,7 @@ __global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_c
     if (tid == 0 && tau_out) *tau_out = top == -INFINITY ? INFINITY : NAN;
     return;
   }
-  const float floor_z = top - 1.f;               // no weight at or below
+  floor_z = fmaxf(floor_z, top - 1.f);           // no weight at or below
 
   // ends of the lists in their concatenation
   int raw = 0;
@@ -375,23 +387,37 @@ __global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_c
 
 struct TreePlan {
   int64_t region;        // entries per row
-  int tiles, rows, sub, row_block, ranges;
+  int tiles, rows, sub, block_rows, row_blocks, ranges;
   int64_t row_bytes;     // workspace per row
   int max_parts;
+  bool mma;              // tensor cores
+  int acc_cols, stages;
 };
 
 static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
   TreePlan p{};
   p.tiles = (int)(((int64_t)max_seq + kTreeTile - 1) / kTreeTile);
   p.rows = tokens * (q_heads / c->kv_heads);
-  p.sub = kSimtWarps;
-  p.row_block = kSimtRows;
+  p.mma = c->dtype != EKV_F32;
+  if (p.mma) {
+    const int blocks = (p.rows + kTmMaxRows - 1) / kTmMaxRows;
+    p.block_rows = ((p.rows + blocks - 1) / blocks + 15) / 16 * 16;
+    p.row_blocks = (p.rows + p.block_rows - 1) / p.block_rows;
+    p.sub = kTmSub;
+    p.ranges = sm_count() / p.row_blocks;                 // one block per SM: its tiles fill the shared memory
+    for (p.acc_cols = 16; p.acc_cols < p.block_rows;) p.acc_cols *= 2;
+    for (p.stages = kTmMaxStages; tm_smem_bytes(p.block_rows, c->head_dim, p.stages) > 227 * 1024;) --p.stages;
+  } else {
+    p.block_rows = kSimtRows;
+    p.row_blocks = (p.rows + kSimtRows - 1) / kSimtRows;
+    p.sub = kSimtWarps;
+    p.ranges = 2 * sm_count() / p.row_blocks;
+  }
+  if (p.ranges < 1) p.ranges = 1;
   // drafted survivors are kept behind the cache's
   p.region = (int64_t)p.tiles * kTreeTile + (tokens + 1) / 2 * 2;
-  const int blocks = (p.rows + p.row_block - 1) / p.row_block;
-  p.ranges = 2 * sm_count() / blocks > 0 ? 2 * sm_count() / blocks : 1;
   p.max_parts = p.ranges < p.tiles ? p.ranges : (p.tiles > 0 ? p.tiles : 1);
-  p.row_bytes = p.region * (int64_t)sizeof(uint2) + 8ll * p.max_parts * p.sub;
+  p.row_bytes = p.region * (int64_t)sizeof(uint2) + 12ll * p.max_parts * p.sub;
   return p;
 }
 
@@ -403,11 +429,32 @@ static int64_t tree_groups_per_turn(const TreePlan& p, int groups) {
   return n < 1 ? 1 : (n > groups ? groups : n);
 }
 
+template <typename T, int D>
+static int launch_scores(const TreeArgs& a, const TreePlan& p, cudaStream_t st) {
+  const unsigned grid = (unsigned)(a.ranges * a.row_blocks);
+  if constexpr (sizeof(T) == 2) {
+    const size_t smem = tm_smem_bytes(p.block_rows, D, p.stages);
+    cudaError_t e = cudaFuncSetAttribute(tree_scores_mma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    tree_scores_mma_kernel<T, D><<<grid, kTmThreads, smem, st>>>(a, p.block_rows, p.acc_cols, p.stages);
+  } else {
+    const size_t smem = sizeof(float) * (kSimtRows + kSimtKeys) * (D + 4);
+    cudaError_t e = cudaFuncSetAttribute(tree_scores_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    tree_scores_simt_kernel<T, D><<<grid, kSimtWarps * 32, smem, st>>>(a);
+  }
+  return EKV_OK;
+}
+
 static bool tree_sizes_ok(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
   return q_heads > 0 && q_heads % c->kv_heads == 0 && tokens > 0 && tokens <= EKV_TREE_MAX_TOKENS && max_seq >= 0 &&
          max_seq <= c->capacity && max_seq <= c->page_capacity * (int64_t)c->page_size &&
          (int64_t)tokens * (q_heads / c->kv_heads) <= (1 << 20) && (int64_t)c->batch * q_heads * tokens <= 0x7fffffff;
 }
+
+unsigned int copy_timeouts_tree() { return copy_timeouts_here(); }
 
 }  // namespace ekv
 
@@ -467,7 +514,7 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   a.row0 = 0;
   a.rows = p.rows;
   a.ranges = p.ranges;
-  a.row_blocks = (p.rows + p.row_block - 1) / p.row_block;
+  a.row_blocks = p.row_blocks;
   a.sub = p.sub;
   a.max_parts = p.max_parts;
   a.region = p.region;
@@ -475,6 +522,7 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   a.entries = static_cast<uint2*>(workspace);
   a.counts = reinterpret_cast<int*>(a.entries + turn * p.rows * p.region);
   a.maxima = reinterpret_cast<float*>(a.counts + turn * p.rows * p.max_parts * p.sub);
+  a.bounds = a.maxima + turn * p.rows * p.max_parts * p.sub;
   const size_t fin_smem = sizeof(int) * ((size_t)p.max_parts * p.sub + 1 + tokens);
   cudaStream_t st = as_stream(stream);
   for (int g0 = 0; g0 < groups; g0 += (int)turn) {
@@ -482,14 +530,10 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
     a.g1 = (int)(g0 + turn < groups ? g0 + turn : groups);
     const int64_t rows = (int64_t)(a.g1 - g0) * p.rows;
     if (rows > 0x7fffffff) return EKV_ERR_ARG;
+    int err = EKV_OK;
     EKV_DISPATCH(c->dtype, c->head_dim, {
-      if (max_seq_len > 0) {
-        const size_t smem = sizeof(float) * (kSimtRows + kSimtKeys) * (D + 4);
-        cudaError_t e = cudaFuncSetAttribute(tree_scores_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)smem);
-        if (e != cudaSuccess) return (int)e;
-        tree_scores_simt_kernel<T, D><<<a.ranges * a.row_blocks, kSimtWarps * 32, smem, st>>>(a);
-      }
+      if (max_seq_len > 0) err = launch_scores<T, D>(a, p, st);
+      if (err) return err;
       tree_finish_kernel<T, D><<<(unsigned)rows, kFinThreads, fin_smem, st>>>(a);
     });
   }

@@ -48,7 +48,9 @@ struct TreeArgs {
   uint2* entries;                      // [groups][rows][region]: z bits, key
   int64_t region;
   int* counts;                         // [groups][rows][max_parts * sub]
-  float* maxima;                       // same shape
+  float* maxima;                       // same shape: largest z of the list's keys
+  float* bounds;                       // same shape: no key of the list's share that lies above is missing from it, and
+                                       // tau lies above
   int* status;
 };
 
