@@ -1,4 +1,6 @@
 // Entmax attention of a tree of drafted tokens over the cache (see ekv_tree.cuh for the method).
+#include <cudaTypedefs.h>
+
 #include "ekv_tree_mma.cuh"
 
 namespace ekv {
@@ -95,13 +97,12 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
       if (lane < live) {
 #pragma unroll
         for (int j = 0; j < KPW; ++j)
-          if (j < valid && acc[j] > top - 1.f) list[count++] = make_uint2(__float_as_uint(acc[j]), key0 + warp * KPW + j);
+          if (j < valid && !(acc[j] <= top - 1.f)) list[count++] = make_uint2(__float_as_uint(acc[j]), key0 + warp * KPW + j);
       }
     }
     if (lane < live) {
       const int64_t at = row_id * a.max_parts * a.sub + part * a.sub + warp;
       a.counts[at] = count;
-      a.maxima[at] = top;
       a.bounds[at] = top - 1.f;
     }
   }
@@ -218,38 +219,15 @@ __global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_c
   const int parts = n_tiles ? split.piece_of(g_first + n_tiles - 1) - piece0 + 1 : 0;
   const int lists = parts * a.sub;
   const int* const counts = a.counts + row_id * a.max_parts * a.sub;
-  const float* const maxima = a.maxima + row_id * a.max_parts * a.sub;
   const float* const bounds = a.bounds + row_id * a.max_parts * a.sub;
-  float top = -INFINITY, floor_z = -INFINITY;
+  float floor_z = -INFINITY;                     // no weight at or below; fmaxf passes over a NaN
   __syncthreads();                               // s_zd
-  for (int i = tid; i < lists; i += kFinThreads) {
-    top = max_nan(top, maxima[i]);
-    floor_z = fmaxf(floor_z, bounds[i]);
-  }
-  for (int j = tid; j < a.tokens; j += kFinThreads) top = max_nan(top, s_zd[j]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int i = tid; i < lists; i += kFinThreads) floor_z = fmaxf(floor_z, bounds[i]);
   floor_z = warp_max(floor_z);
-  if (lane == 0) {
-    scratch[warp] = top;
-    scratch[8 + warp] = floor_z;
-  }
+  if (lane == 0) scratch[warp] = floor_z;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kFinThreads / 32; ++w) {
-    top = max_nan(top, scratch[w]);
-    floor_z = fmaxf(floor_z, scratch[8 + w]);
-  }
-
-  T* const out = static_cast<T*>(a.out) + b * a.os[0] + hq * a.os[1] + t * a.os[2];
-  float* const tau_out = a.tau ? a.tau + ((int64_t)b * a.q_heads + hq) * a.tokens + t : nullptr;
-  if (!(fabsf(top) < INFINITY)) {                // nothing visible: zeros.  NaN or +inf among the scores: NaN
-    const float fill = top == -INFINITY ? 0.f : NAN;
-    if (tid < D) out[tid] = from_float<T>(fill);
-    if (tid == 0 && tau_out) *tau_out = top == -INFINITY ? INFINITY : NAN;
-    return;
-  }
-  floor_z = fmaxf(floor_z, top - 1.f);           // no weight at or below
+  for (int w = 0; w < kFinThreads / 32; ++w) floor_z = fmaxf(floor_z, scratch[w]);
 
   // ends of the lists in their concatenation
   int raw = 0;
@@ -262,8 +240,9 @@ __global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_c
   }
   __syncthreads();
 
-  // what the final maximum leaves, in order
+  // what the largest bound leaves, in order; a NaN stays
   int n = 0;
+  float top = -INFINITY;
   for (int i0 = 0; i0 < raw; i0 += kFinThreads * kFinPer) {
     uint2 e[kFinPer];
     int keep = 0, mine = 0;
@@ -284,9 +263,10 @@ __global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_c
           const int64_t hi_t = min(split.begin(piece0 + p + 1), g_first + n_tiles) - g_first;
           const int64_t base = lo_t * kTreeTile + s * (hi_t - lo_t) * (kTreeTile / a.sub);
           e[j] = row.region[base + (i + j - (l ? s_end[l - 1] : 0))];
-          if (__uint_as_float(e[j].x) > floor_z) {
+          if (!(__uint_as_float(e[j].x) <= floor_z)) {
             keep |= 1 << j;
             ++mine;
+            top = max_nan(top, __uint_as_float(e[j].x));
           }
         }
       }
@@ -301,13 +281,29 @@ __global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_c
   }
   for (int j0 = 0; j0 < a.tokens; j0 += kFinThreads) {
     const int j = j0 + tid;
-    const bool keep = j < a.tokens && s_zd[j] > floor_z;
+    const bool keep = j < a.tokens && !(s_zd[j] <= floor_z);             // -inf: not seen
+    if (keep) top = max_nan(top, s_zd[j]);
     int all;
     const int at = n + block_excl(keep, reinterpret_cast<int*>(scratch), &all);
     if (keep) row.put(at, make_uint2(__float_as_uint(s_zd[j]), ~j));     // a negative key: drafted
     n += all;
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   __syncthreads();
+  if (lane == 0) scratch[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kFinThreads / 32; ++w) top = max_nan(top, scratch[w]);
+  T* const out = static_cast<T*>(a.out) + b * a.os[0] + hq * a.os[1] + t * a.os[2];
+  float* const tau_out = a.tau ? a.tau + ((int64_t)b * a.q_heads + hq) * a.tokens + t : nullptr;
+  if (!(fabsf(top) < INFINITY)) {                // nothing visible: zeros.  NaN or +inf among the scores: NaN
+    const float fill = top == -INFINITY ? 0.f : NAN;
+    if (tid < D) out[tid] = from_float<T>(fill);
+    if (tid == 0 && tau_out) *tau_out = top == -INFINITY ? INFINITY : NAN;
+    return;
+  }
+  floor_z = fmaxf(floor_z, top - 1.f);
 
   // tau: the norm N(tau) = (sum (z - tau)_+^beta)^(1/beta) falls to 1 at the root and is convex for beta >= 1 (nearly
   // linear when the support is settled), so Newton's steps on it from max - 1 climb towards the root from the left;
@@ -387,38 +383,80 @@ __global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_c
 
 struct TreePlan {
   int64_t region;        // entries per row
-  int tiles, rows, sub, block_rows, row_blocks, ranges;
+  int tiles, rows, sub, row_blocks, ranges, tile_keys;
   int64_t row_bytes;     // workspace per row
   int max_parts;
-  bool mma;              // tensor cores
-  int acc_cols, stages;
+  bool mma, sample;      // tensor cores; a sample before the pass
+  int sample_tiles;
+  TmShape shape;
 };
+
+constexpr int kSampleFrom = 8;         // tiles per block from which on there is a sample
 
 static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
   TreePlan p{};
-  p.tiles = (int)(((int64_t)max_seq + kTreeTile - 1) / kTreeTile);
   p.rows = tokens * (q_heads / c->kv_heads);
   p.mma = c->dtype != EKV_F32;
+  p.tile_keys = kTreeTile;
   if (p.mma) {
+    TmShape& sh = p.shape;
     const int blocks = (p.rows + kTmMaxRows - 1) / kTmMaxRows;
-    p.block_rows = ((p.rows + blocks - 1) / blocks + 15) / 16 * 16;
-    p.row_blocks = (p.rows + p.block_rows - 1) / p.block_rows;
+    sh.n_rows = ((p.rows + blocks - 1) / blocks + 15) / 16 * 16;
+    p.row_blocks = (p.rows + sh.n_rows - 1) / sh.n_rows;
     p.sub = kTmSub;
     p.ranges = sm_count() / p.row_blocks;                 // one block per SM: its tiles fill the shared memory
-    for (p.acc_cols = 16; p.acc_cols < p.block_rows;) p.acc_cols *= 2;
-    for (p.stages = kTmMaxStages; tm_smem_bytes(p.block_rows, c->head_dim, p.stages) > 227 * 1024;) --p.stages;
+    for (sh.acc_cols = 16; sh.acc_cols < sh.n_rows;) sh.acc_cols *= 2;
+    for (sh.stages = kTmMaxStages; tm_smem_bytes(sh.n_rows, c->head_dim, sh.stages) > 227 * 1024;) --sh.stages;
+    // a copy must not cross a page: the largest divisor of the page size that fits a tile
+    sh.box_rows = kTreeTile;
+    if (c->block_table)
+      while (c->page_size % sh.box_rows) --sh.box_rows;
+    p.tile_keys = kTreeTile / sh.box_rows * sh.box_rows;
   } else {
-    p.block_rows = kSimtRows;
     p.row_blocks = (p.rows + kSimtRows - 1) / kSimtRows;
     p.sub = kSimtWarps;
     p.ranges = 2 * sm_count() / p.row_blocks;
   }
   if (p.ranges < 1) p.ranges = 1;
+  p.tiles = (int)(((int64_t)max_seq + p.tile_keys - 1) / p.tile_keys);
   // drafted survivors are kept behind the cache's
   p.region = (int64_t)p.tiles * kTreeTile + (tokens + 1) / 2 * 2;
   p.max_parts = p.ranges < p.tiles ? p.ranges : (p.tiles > 0 ? p.tiles : 1);
-  p.row_bytes = p.region * (int64_t)sizeof(uint2) + 12ll * p.max_parts * p.sub;
+  p.row_bytes = p.region * (int64_t)sizeof(uint2) + 8ll * p.max_parts * p.sub;
+  if (p.mma && (int64_t)p.tiles * c->batch * c->kv_heads >= (int64_t)kSampleFrom * p.ranges) {
+    p.sample = true;
+    p.sample_tiles = (p.tiles + kSampleStride - 1) / kSampleStride;
+    if (p.sample_tiles > kSampleTiles) p.sample_tiles = kSampleTiles;
+    p.row_bytes += 16ll * p.sample_tiles;
+  }
   return p;
+}
+
+// K as the copies see it: [blocks or sequences][KV heads][rows][D]
+static int tree_k_map(CUtensorMap* map, const ekv_cache_desc* c, int box_rows) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return (int)e;
+    if (found != cudaDriverEntryPointSuccess) return (int)cudaErrorNotSupported;
+    encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }
+  const bool paged = c->block_table != nullptr;
+  const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)(paged ? c->page_size : c->capacity),
+                              (cuuint64_t)c->kv_heads, (cuuint64_t)(paged ? c->num_blocks : c->batch)};
+  // the stride of an axis of one entry may be anything
+  const cuuint64_t row = (cuuint64_t)c->head_dim * 2;
+  const cuuint64_t head = c->kv_heads > 1 ? (cuuint64_t)c->kv_stride_h * 2 : row * dims[1];
+  const cuuint64_t block = dims[3] > 1 ? (cuuint64_t)(paged ? c->kv_stride_block : c->kv_stride_b) * 2 : head * dims[2];
+  const cuuint64_t strides[3] = {row, head, block};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, unit[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, c->dtype == EKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            4, c->k, dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? EKV_OK : EKV_ERR_ARG;
 }
 
 // what a launch may use of the GPU's memory before the groups are taken in several turns
@@ -430,14 +468,16 @@ static int64_t tree_groups_per_turn(const TreePlan& p, int groups) {
 }
 
 template <typename T, int D>
-static int launch_scores(const TreeArgs& a, const TreePlan& p, cudaStream_t st) {
+static int launch_scores(const TreeArgs& a, const TreePlan& p, const CUtensorMap& k_map, cudaStream_t st) {
   const unsigned grid = (unsigned)(a.ranges * a.row_blocks);
   if constexpr (sizeof(T) == 2) {
-    const size_t smem = tm_smem_bytes(p.block_rows, D, p.stages);
-    cudaError_t e = cudaFuncSetAttribute(tree_scores_mma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
+    const int smem = (int)tm_smem_bytes(p.shape.n_rows, D, p.shape.stages);
+    const auto pass = tree_scores_mma_kernel<T, D, false>, sample = tree_scores_mma_kernel<T, D, true>;
+    cudaError_t e = cudaFuncSetAttribute(pass, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(sample, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
-    tree_scores_mma_kernel<T, D><<<grid, kTmThreads, smem, st>>>(a, p.block_rows, p.acc_cols, p.stages);
+    if (p.sample) sample<<<grid, kTmThreads, smem, st>>>(a, k_map, p.shape);
+    pass<<<grid, kTmThreads, smem, st>>>(a, k_map, p.shape);
   } else {
     const size_t smem = sizeof(float) * (kSimtRows + kSimtKeys) * (D + 4);
     cudaError_t e = cudaFuncSetAttribute(tree_scores_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -521,10 +561,16 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   a.status = status;
   a.entries = static_cast<uint2*>(workspace);
   a.counts = reinterpret_cast<int*>(a.entries + turn * p.rows * p.region);
-  a.maxima = reinterpret_cast<float*>(a.counts + turn * p.rows * p.max_parts * p.sub);
-  a.bounds = a.maxima + turn * p.rows * p.max_parts * p.sub;
+  a.bounds = reinterpret_cast<float*>(a.counts + turn * p.rows * p.max_parts * p.sub);
+  a.classes = a.bounds + turn * p.rows * p.max_parts * p.sub;
+  a.sample = p.sample;
+  a.sample_tiles = p.sample_tiles;
+  a.tile_keys = p.tile_keys;
   const size_t fin_smem = sizeof(int) * ((size_t)p.max_parts * p.sub + 1 + tokens);
   cudaStream_t st = as_stream(stream);
+  CUtensorMap k_map{};
+  if (p.mma && max_seq_len > 0)
+    if (int e = tree_k_map(&k_map, c, p.shape.box_rows)) return e;
   for (int g0 = 0; g0 < groups; g0 += (int)turn) {
     a.g0 = g0;
     a.g1 = (int)(g0 + turn < groups ? g0 + turn : groups);
@@ -532,7 +578,7 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
     if (rows > 0x7fffffff) return EKV_ERR_ARG;
     int err = EKV_OK;
     EKV_DISPATCH(c->dtype, c->head_dim, {
-      if (max_seq_len > 0) err = launch_scores<T, D>(a, p, st);
+      if (max_seq_len > 0) err = launch_scores<T, D>(a, p, k_map, st);
       if (err) return err;
       tree_finish_kernel<T, D><<<(unsigned)rows, kFinThreads, fin_smem, st>>>(a);
     });
