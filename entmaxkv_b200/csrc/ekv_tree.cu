@@ -22,10 +22,9 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int range = blockIdx.x / a.row_blocks, rb = blockIdx.x % a.row_blocks;
   const int H = a.c.kv_heads;
-  const TreeSplit split = tree_split(tree_tiles_before(a, a.g1, lane), a.ranges);
-  if (split.W == 0 || range >= split.N) return;
-  const int64_t t_begin = split.begin(range), t_end = split.begin(range + 1);
-  const TreeAt at = tree_find(a, t_begin, lane);
+  const TreeRange at = tree_range<false>(a, range, lane);
+  if (at.t_begin == at.t_end) return;
+  const int64_t t_begin = at.t_begin, t_end = at.t_end;
   int64_t g_first = at.first;                           // first tile of the group
   for (int g = at.g; g < a.g1 && g_first < t_end; ++g) {
     const int b = g / H, hkv = g % H;
@@ -33,7 +32,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
     if (n == 0) continue;
     const int64_t g_end = g_first + n;
     const int tile0 = (int)(max(t_begin, g_first) - g_first), tile1 = (int)(min(t_end, g_end) - g_first);
-    const int part = range - split.piece_of(g_first);
+    const int part = range - at.split.piece_of(g_first);
     const int len = tree_len(a, b);
     const int live = min(tree_drafts(a, b) * a.group - a.row0, a.rows) - rb * kSimtRows;   // rows of this block
     g_first = g_end;
@@ -53,8 +52,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
       for (int j = 0; j < EPL; ++j) s_q[row * PITCH + e + j] = x[j];
     }
     const int64_t row_id = (int64_t)(g - a.g0) * a.rows + rb * kSimtRows + lane;
-    uint2* const list = a.entries + row_id * a.region + (int64_t)tile0 * kTreeTile +
-                        (int64_t)warp * (tile1 - tile0) * (kTreeTile / kSimtWarps);
+    uint2* const list = a.entries + row_id * a.region + tree_list_place(a, tile0, part, tile1 - tile0, warp);
     int count = 0;
     float top = -INFINITY;
     for (int key0 = tile0 * kTreeTile; key0 < min(tile1 * kTreeTile, len); key0 += kSimtKeys) {
@@ -108,47 +106,138 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
   }
 }
 
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // ---- tau and output ------------------------------------------------------------------------------------------------
+//
+// A warp per row while at most 512 candidates lie above the row's best bound (the usual case: no barrier, sums by
+// shuffle), the whole block per row where more do (flat scores), one such row after another.
 
-constexpr int kFinThreads = 256;
-constexpr int kFinSlots = 2048;        // survivors in shared memory; more stay in the row's region
-constexpr int kFinPer = 4;             // list entries per thread and round
+constexpr int kFinThreads = 256, kFinWarps = kFinThreads / 32;
+constexpr int kFinLight = 512;                  // survivors of a row that one warp finishes
+constexpr int kFinLists = 256;                  // and its lists
+constexpr int kFinSlots = kFinWarps * kFinLight;   // of a heavy row on chip; more stay in the row's region
 
+// What both ways need to know about a row.
 struct FinRow {
-  float* z;                            // [kFinSlots]
-  int* key;
+  int b, hkv, hq, t, drafts;
+  int64_t id;
+  int64_t first;                                // the group's first tile
+  int tiles, piece0, lists, len;
+  TreeSplit split;
   uint2* region;
-  __device__ __forceinline__ uint2 get(int i) const {
-    return i < kFinSlots ? make_uint2(__float_as_uint(z[i]), (uint32_t)key[i]) : region[i];
-  }
-  __device__ __forceinline__ void put(int i, uint2 e) const {
-    if (i < kFinSlots) {
-      z[i] = __uint_as_float(e.x);
-      key[i] = (int)e.y;
-    } else {
-      region[i] = e;
-    }
-  }
 };
+__device__ __forceinline__ FinRow fin_row(const TreeArgs& a, int64_t id, int lane) {
+  FinRow r;
+  r.id = id;
+  const int g = a.g0 + (int)(id / a.rows), row = a.row0 + (int)(id % a.rows);
+  r.b = g / a.c.kv_heads;
+  r.hkv = g % a.c.kv_heads;
+  r.hq = r.hkv * a.group + row % a.group;
+  r.t = row / a.group;
+  r.drafts = tree_drafts(a, r.b);
+  r.len = tree_len(a, r.b);
+  r.lists = 0;
+  r.region = a.entries + id * a.region;
+  if (a.dense) return r;
+  const TreeGroup at = tree_group(a, g, lane);
+  r.split = at.split;
+  r.first = at.first;
+  r.tiles = tree_tiles(a, r.b);
+  r.piece0 = r.tiles ? r.split.piece_of(r.first) : 0;
+  r.lists = r.tiles ? (r.split.piece_of(r.first + r.tiles - 1) - r.piece0 + 1) * a.sub : 0;
+  return r;
+}
+// entry i of the concatenation of the row's lists, which end at ends[] (or of all its scores)
+__device__ __forceinline__ uint2 fin_entry(const TreeArgs& a, const FinRow& r, const int* ends, int i) {
+  if (a.dense) return make_uint2(__float_as_uint(reinterpret_cast<const float*>(r.region)[a.region + i]), (uint32_t)i);
+  int lo = 0, hi = r.lists - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ends[mid] > i) hi = mid; else lo = mid + 1;
+  }
+  const int p = lo / a.sub, s = lo % a.sub;
+  const int64_t t0 = max(r.split.begin(r.piece0 + p), r.first) - r.first;
+  const int64_t t1 = min(r.split.begin(r.piece0 + p + 1), r.first + r.tiles) - r.first;
+  return r.region[tree_list_place(a, t0, p, t1 - t0, s) + (i - (lo ? ends[lo - 1] : 0))];
+}
+// 16 bytes of the value row of a key (or, ~j, of a drafted token)
+template <typename T, int D>
+__device__ __forceinline__ uint4 fin_value(const TreeArgs& a, const FinRow& r, int key, int col) {
+  const T* v;
+  if (key < 0) {
+    v = static_cast<const T*>(a.v_draft) + r.b * a.vs[0] + r.hkv * a.vs[1] + (int64_t)~key * a.vs[2];
+  } else {
+    int page, in_page;
+    size_t off;
+    a.by_page.divmod(key, page, in_page);
+    if (!kv_page_offset(a.c, r.b, r.hkv, page, off)) return make_uint4(0, 0, 0, 0);
+    v = static_cast<const T*>(a.c.v) + off + (size_t)in_page * D;
+  }
+  return *reinterpret_cast<const uint4*>(v + col);
+}
+// Scores of the drafted keys that the row sees (-inf: not), `groups` sets of LPR lanes side by side, this one `mine`.
+template <typename T, int D>
+__device__ __forceinline__ void fin_drafts(const TreeArgs& a, const FinRow& r, float* zd, int mine, int groups, int lane) {
+  constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL;
+  const int col = lane % LPR * EPL;
+  float q[EPL];
+  unpack<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + r.b * a.qs[0] + r.hq * a.qs[1] + r.t * a.qs[2] + col), q);
+  const unsigned char* const seen = a.mask + r.b * a.ms_b + r.t * a.ms_t;
+  const T* const k0 = static_cast<const T*>(a.k_draft) + r.b * a.ks[0] + r.hkv * a.ks[1] + col;
+#pragma unroll 4
+  for (int j0 = 0; j0 < a.tokens; j0 += groups) {
+    const int j = j0 + mine;
+    const bool sees = j < r.drafts && seen[j];
+    float k[EPL], s = 0.f;
+    unpack<T>(sees ? *reinterpret_cast<const uint4*>(k0 + j * a.ks[2]) : make_uint4(0, 0, 0, 0), k);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) s = fmaf(q[e], k[e], s);
+    s = row_sum<LPR>(s);
+    if (lane % LPR == 0 && j < a.tokens) zd[j] = sees ? s * a.zscale : -INFINITY;
+  }
+}
 
-__device__ __forceinline__ float3 block_sum3(float3 v, float* scratch) {
+// Root of sum (z - tau)_+^beta = 1 from below.  The norm N(tau) = (sum (z - tau)_+^beta)^(1/beta) falls to 1 at the root and
+// is convex for beta >= 1 (nearly linear when the support is settled), so Newton's steps on it climb towards the root from
+// the left; the bracket keeps them safe for beta < 1.  `sums(tau)` gives sum d^beta and sum d^(beta-1) to every thread.
+template <typename Sums>
+__device__ __forceinline__ float fin_tau(float floor_z, float top, float alpha, int kind, Sums sums) {
+  float lo = floor_z, hi = top, tau = floor_z;
+  for (int it = 0; it < 40; ++it) {
+    const float2 s = sums(tau);
+    if (s.x >= 1.f) lo = tau; else hi = tau;
+    // (N - 1) / -N' = (s0^(1/beta) - 1) s0^(1 - 1/beta) / s1
+    const float root = kind == 0 ? s.x : (kind == 1 ? sqrtf(s.x) : pow_pos(s.x, alpha - 1.f));
+    const float step = s.x > 0.f ? (root - 1.f) * (s.x / root) / s.y : -INFINITY;
+    // half a unit in the last place of the scores that tau is compared with
+    const bool done = fabsf(step) <= 6e-8f * fmaxf(fabsf(tau), fabsf(top));
+    const float next = tau + step;
+    tau = next > lo && next < hi ? next : (done ? tau : 0.5f * (lo + hi));
+    if (done) break;
+  }
+  return tau;
+}
+
+__device__ __forceinline__ float2 block_sum2(float2 v, float* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v.x = warp_sum(v.x);
   v.y = warp_sum(v.y);
-  v.z = warp_sum(v.z);
   __syncthreads();
   if (lane == 0) {
-    scratch[warp * 3] = v.x;
-    scratch[warp * 3 + 1] = v.y;
-    scratch[warp * 3 + 2] = v.z;
+    scratch[warp * 2] = v.x;
+    scratch[warp * 2 + 1] = v.y;
   }
   __syncthreads();
-  float3 t = make_float3(0.f, 0.f, 0.f);
+  float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < kFinThreads / 32; ++w) {
-    t.x += scratch[w * 3];
-    t.y += scratch[w * 3 + 1];
-    t.z += scratch[w * 3 + 2];
+  for (int w = 0; w < kFinWarps; ++w) {
+    t.x += scratch[w * 2];
+    t.y += scratch[w * 2 + 1];
   }
   return t;
 }
@@ -167,7 +256,7 @@ __device__ __forceinline__ int block_excl(int v, int* scratch, int* total) {
   __syncthreads();
   int base = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kFinThreads / 32; ++w) {
+  for (int w = 0; w < kFinWarps; ++w) {
     if (w < warp) base += scratch[w];
     all += scratch[w];
   }
@@ -175,238 +264,321 @@ __device__ __forceinline__ int block_excl(int v, int* scratch, int* total) {
   return base + inc - v;
 }
 
+// Survivors of a heavy row: the first kFinSlots on chip, the others over the row's lists (in place: what is written at i
+// was entry i or a later one).
+struct FinHeavy {
+  uint2* slots;
+  uint2* region;
+  __device__ __forceinline__ uint2 get(int i) const { return i < kFinSlots ? slots[i] : region[i]; }
+  __device__ __forceinline__ void put(int i, uint2 e) const { (i < kFinSlots ? slots[i] : region[i]) = e; }
+};
+
+// list ends in shared memory: kFinLists per warp, or all lists of one row
+static inline int fin_ends(int max_lists) {
+  const int each = max_lists < kFinLists ? max_lists : kFinLists;
+  return each * kFinWarps > max_lists ? each * kFinWarps : max_lists;
+}
+
+// dynamic shared memory: [n_ends] list ends, [warps][tokens] drafted scores
 template <typename T, int D>
-__global__ void __launch_bounds__(kFinThreads) tree_finish_kernel(const __grid_constant__ TreeArgs a) {
-  constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL, GROUPS = kFinThreads / LPR;
-  __shared__ float s_z[kFinSlots];
-  __shared__ int s_key[kFinSlots];
+__global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __grid_constant__ TreeArgs a, const int64_t n_rows,
+                                                                     const int n_ends) {
+  constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL, SIDE = 32 / LPR, GROUPS = kFinThreads / LPR;
+  __shared__ uint2 s_slots[kFinSlots];
   __shared__ float scratch[32];
-  __shared__ float s_acc[GROUPS * D];
-  extern __shared__ int s_dyn[];                 // [parts * sub + 1] list ends, [tokens] drafted scores
+  __shared__ int s_heavy[kFinWarps];
+  extern __shared__ int s_dyn[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int H = a.c.kv_heads;
-  const int gl = blockIdx.x / a.rows, rl = blockIdx.x % a.rows;
-  const int g = a.g0 + gl, r = a.row0 + rl;
-  const int b = g / H, hkv = g % H, hq = hkv * a.group + r % a.group, t = r / a.group;
-  const int drafts = tree_drafts(a, b);
-  if (t >= drafts) return;                       // behind a short tree: left as it was
-  const int64_t row_id = (int64_t)gl * a.rows + rl;
-  int* const s_end = s_dyn;
-  float* const s_zd = reinterpret_cast<float*>(s_dyn + a.max_parts * a.sub + 1);
-  const FinRow row{s_z, s_key, a.entries + row_id * a.region};
+  int* const ends = s_dyn + warp * min(a.max_parts * a.sub, kFinLists);
+  float* const zd = reinterpret_cast<float*>(s_dyn + n_ends) + warp * a.tokens;
+  const int64_t id0 = (int64_t)blockIdx.x * kFinWarps;
+  const int kind = alpha_kind_of(a.alpha);
+  const float beta = 1.f / (a.alpha - 1.f);
 
-  // drafted keys: a warp per key
-  {
-    const T* const qrow = static_cast<const T*>(a.q) + b * a.qs[0] + hq * a.qs[1] + t * a.qs[2];
-    const unsigned char* const seen = a.mask + b * a.ms_b + t * a.ms_t;
-    for (int j = warp; j < a.tokens; j += kFinThreads / 32) {
-      float s = -INFINITY;
-      if (j < drafts && seen[j]) {
-        const T* const krow = static_cast<const T*>(a.k_draft) + b * a.ks[0] + hkv * a.ks[1] + j * a.ks[2];
-        s = 0.f;
+  FinRow r{};
+  bool mine = id0 + warp < n_rows, heavy = false;
+  if (mine) {
+    r = fin_row(a, id0 + warp, lane);
+    mine = r.t < r.drafts;                       // else behind a short tree: left as it was
+  }
+  float floor_z = -INFINITY, top = -INFINITY;    // no weight at or below the floor; fmaxf passes over a NaN
+  int raw = r.len, n = 0;
+  uint2* const slots = s_slots + warp * kFinLight;
+  if (mine) {
+    if (!a.dense && r.lists > kFinLists) {
+      n = kFinLight + 1;                         // the block's
+    } else if (!a.dense) {
+      raw = 0;
+      const int* const counts = a.counts + r.id * a.max_parts * a.sub;
+      const float* const bounds = a.bounds + r.id * a.max_parts * a.sub;
+      for (int i0 = 0; i0 < r.lists; i0 += 32) {
+        const bool in = i0 + lane < r.lists;
+        int end = in ? counts[i0 + lane] : 0;
+        if (in) floor_z = fmaxf(floor_z, bounds[i0 + lane]);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) s = fmaf(to_float<T>(qrow[lane + 32 * e]), to_float<T>(krow[lane + 32 * e]), s);
-        s = warp_sum(s) * a.zscale;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int m = __shfl_up_sync(0xffffffffu, end, o);
+          if (lane >= o) end += m;
+        }
+        if (in) ends[i0 + lane] = raw + end;
+        raw += __shfl_sync(0xffffffffu, end, 31);
       }
-      if (lane == 0) s_zd[j] = s;
+      floor_z = warp_max(floor_z);
     }
-  }
-  // the pieces that hold this group's lists
-  const int64_t W = tree_tiles_before(a, a.g1, lane), g_first = tree_tiles_before(a, g, lane);
-  const int n_tiles = tree_tiles(a, b);
-  const TreeSplit split = tree_split(W, a.ranges);
-  const int piece0 = n_tiles ? split.piece_of(g_first) : 0;
-  const int parts = n_tiles ? split.piece_of(g_first + n_tiles - 1) - piece0 + 1 : 0;
-  const int lists = parts * a.sub;
-  const int* const counts = a.counts + row_id * a.max_parts * a.sub;
-  const float* const bounds = a.bounds + row_id * a.max_parts * a.sub;
-  float floor_z = -INFINITY;                     // no weight at or below; fmaxf passes over a NaN
-  __syncthreads();                               // s_zd
-  for (int i = tid; i < lists; i += kFinThreads) floor_z = fmaxf(floor_z, bounds[i]);
-  floor_z = warp_max(floor_z);
-  if (lane == 0) scratch[warp] = floor_z;
-  __syncthreads();
+    fin_drafts<T, D>(a, r, zd, lane / LPR, SIDE, lane);
+    __syncwarp();
+    if (a.dense) {                               // nothing bounds tau yet: the maximum first
+      const float* const z = reinterpret_cast<const float*>(r.region) + a.region;
+#pragma unroll 8
+      for (int i = lane; i < raw; i += 32) top = max_nan(top, z[i]);
+      for (int j = lane; j < a.tokens; j += 32) top = max_nan(top, zd[j]);
+      top = warp_max_nan(top);
+      floor_z = top - 1.f;
+    }
+    // what lies above the floor, in order; a NaN stays
+    constexpr int AT_ONCE = 4;
+    for (int i0 = 0; i0 < raw + a.tokens && n <= kFinLight; i0 += 32 * AT_ONCE) {
+      uint2 e[AT_ONCE];
 #pragma unroll
-  for (int w = 0; w < kFinThreads / 32; ++w) floor_z = fmaxf(floor_z, scratch[w]);
-
-  // ends of the lists in their concatenation
-  int raw = 0;
-  for (int i0 = 0; i0 < lists; i0 += kFinThreads) {
-    int all;
-    const int n = i0 + tid < lists ? counts[i0 + tid] : 0;
-    const int ex = block_excl(n, reinterpret_cast<int*>(scratch), &all);
-    if (i0 + tid < lists) s_end[i0 + tid] = raw + ex + n;
-    raw += all;
-  }
-  __syncthreads();
-
-  // what the largest bound leaves, in order; a NaN stays
-  int n = 0;
-  float top = -INFINITY;
-  for (int i0 = 0; i0 < raw; i0 += kFinThreads * kFinPer) {
-    uint2 e[kFinPer];
-    int keep = 0, mine = 0;
-    int i = i0 + tid * kFinPer;
-    if (i < raw) {
-      int lo = 0, hi = lists - 1;                // the list that holds entry i
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s_end[mid] > i) hi = mid; else lo = mid + 1;
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int i = i0 + 32 * k + lane;
+        e[k] = make_uint2(__float_as_uint(-INFINITY), 0);
+        if (i < raw) e[k] = fin_entry(a, r, ends, i);
+        else if (i < raw + a.tokens) e[k] = make_uint2(__float_as_uint(zd[i - raw]), (uint32_t)~(i - raw));   // ~j: drafted
       }
-      int l = lo;
 #pragma unroll
-      for (int j = 0; j < kFinPer; ++j) {
-        if (i + j < raw) {
-          while (s_end[l] <= i + j) ++l;
-          const int p = l / a.sub, s = l % a.sub;
-          const int64_t lo_t = max(split.begin(piece0 + p), g_first) - g_first;
-          const int64_t hi_t = min(split.begin(piece0 + p + 1), g_first + n_tiles) - g_first;
-          const int64_t base = lo_t * kTreeTile + s * (hi_t - lo_t) * (kTreeTile / a.sub);
-          e[j] = row.region[base + (i + j - (l ? s_end[l - 1] : 0))];
-          if (!(__uint_as_float(e[j].x) <= floor_z)) {
-            keep |= 1 << j;
-            ++mine;
-            top = max_nan(top, __uint_as_float(e[j].x));
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const float z = __uint_as_float(e[k].x);
+        const bool keep = !(z <= floor_z);
+        const unsigned has = __ballot_sync(0xffffffffu, keep);
+        const int to = n + __popc(has & ((1u << lane) - 1));
+        if (keep) {
+          top = max_nan(top, z);
+          if (to < kFinLight) slots[to] = e[k];
+        }
+        n += __popc(has);
+      }
+    }
+    top = warp_max_nan(top);
+    heavy = n > kFinLight;
+    __syncwarp();
+  }
+  if (lane == 0) s_heavy[warp] = heavy;
+  const auto write = [&](int e, float x) {
+    static_cast<T*>(a.out)[r.b * a.os[0] + r.hq * a.os[1] + r.t * a.os[2] + e] = from_float<T>(x);
+  };
+  const auto write_tau = [&](float x) {
+    if (a.tau) a.tau[((int64_t)r.b * a.q_heads + r.hq) * a.tokens + r.t] = x;
+  };
+
+  if (mine && !heavy) {
+    // ---- a warp per row
+    if (!(fabsf(top) < INFINITY)) {              // nothing visible: zeros.  NaN or +inf among the scores: NaN
+      const float fill = top == -INFINITY ? 0.f : NAN;
+      for (int e = lane; e < D; e += 32) write(e, fill);
+      if (lane == 0) write_tau(top == -INFINITY ? INFINITY : NAN);
+    } else {
+      const float tau = fin_tau(fmaxf(floor_z, top - 1.f), top, a.alpha, kind, [&](float t) {
+        float2 s = make_float2(0.f, 0.f);
+        float s2 = 0.f;
+#pragma unroll 4
+        for (int i = lane; i < n; i += 32)
+          halley_accumulate(__uint_as_float(slots[i].x), t, kind, beta, s.x, s.y, s2);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+          s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+        }
+        return s;
+      });
+      // the support, in order and in place
+      int m = 0;
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        uint2 e = make_uint2(0, 0);
+        float w = 0.f;
+        if (i0 + lane < n) {
+          e = slots[i0 + lane];
+          w = entmax_weight(__uint_as_float(e.x), tau, kind, beta);
+        }
+        const unsigned has = __ballot_sync(0xffffffffu, w > 0.f);
+        if (w > 0.f) slots[m + __popc(has & ((1u << lane) - 1))] = make_uint2(__float_as_uint(w), e.y);
+        m += __popc(has);
+        __syncwarp();
+      }
+      float acc[EPL] = {};
+      const int col = lane % LPR * EPL;
+      constexpr int FLIGHT = 4;
+      for (int i0 = lane / LPR; i0 < m; i0 += SIDE * FLIGHT) {
+        uint4 v[FLIGHT];
+        float w[FLIGHT];
+#pragma unroll
+        for (int f = 0; f < FLIGHT; ++f) {
+          const int i = i0 + f * SIDE;
+          w[f] = 0.f;
+          v[f] = make_uint4(0, 0, 0, 0);
+          if (i < m) {
+            const uint2 e = slots[i];
+            w[f] = __uint_as_float(e.x);
+            v[f] = fin_value<T, D>(a, r, (int)e.y, col);
           }
         }
+#pragma unroll
+        for (int f = 0; f < FLIGHT; ++f)
+          if (i0 + f * SIDE < m) {
+            float x[EPL];
+            unpack<T>(v[f], x);
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) acc[j] = fmaf(w[f], x[j], acc[j]);
+          }
       }
+#pragma unroll
+      for (int o = LPR; o < 32; o <<= 1)
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+      if (lane < LPR)
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) write(col + j, acc[j]);
+      if (lane == 0) write_tau(tau);
     }
-    int all;
-    int at = n + block_excl(mine, reinterpret_cast<int*>(scratch), &all);
-#pragma unroll
-    for (int j = 0; j < kFinPer; ++j)
-      if (keep >> j & 1) row.put(at++, e[j]);
-    n += all;
-    __syncthreads();
-  }
-  for (int j0 = 0; j0 < a.tokens; j0 += kFinThreads) {
-    const int j = j0 + tid;
-    const bool keep = j < a.tokens && !(s_zd[j] <= floor_z);             // -inf: not seen
-    if (keep) top = max_nan(top, s_zd[j]);
-    int all;
-    const int at = n + block_excl(keep, reinterpret_cast<int*>(scratch), &all);
-    if (keep) row.put(at, make_uint2(__float_as_uint(s_zd[j]), ~j));     // a negative key: drafted
-    n += all;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  __syncthreads();
-  if (lane == 0) scratch[warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kFinThreads / 32; ++w) top = max_nan(top, scratch[w]);
-  T* const out = static_cast<T*>(a.out) + b * a.os[0] + hq * a.os[1] + t * a.os[2];
-  float* const tau_out = a.tau ? a.tau + ((int64_t)b * a.q_heads + hq) * a.tokens + t : nullptr;
-  if (!(fabsf(top) < INFINITY)) {                // nothing visible: zeros.  NaN or +inf among the scores: NaN
-    const float fill = top == -INFINITY ? 0.f : NAN;
-    if (tid < D) out[tid] = from_float<T>(fill);
-    if (tid == 0 && tau_out) *tau_out = top == -INFINITY ? INFINITY : NAN;
-    return;
-  }
-  floor_z = fmaxf(floor_z, top - 1.f);
-
-  // tau: the norm N(tau) = (sum (z - tau)_+^beta)^(1/beta) falls to 1 at the root and is convex for beta >= 1 (nearly
-  // linear when the support is settled), so Newton's steps on it from max - 1 climb towards the root from the left;
-  // the bracket keeps them safe for beta < 1.
-  const float beta = 1.f / (a.alpha - 1.f);
-  const int kind = alpha_kind_of(a.alpha);
-  float lo = floor_z, hi = top, tau = floor_z;
-  for (int it = 0; it < 40; ++it) {
-    float3 s = make_float3(0.f, 0.f, 0.f);
-    for (int i = tid; i < n; i += kFinThreads)
-      halley_accumulate(__uint_as_float(row.get(i).x), tau, kind, beta, s.x, s.y, s.z);
-    s = block_sum3(s, scratch);
-    if (s.x >= 1.f) lo = tau; else hi = tau;
-    // N - 1 over -N' = (s0^(1/beta) - 1) s0^(1 - 1/beta) / s1
-    const float root = kind == 0 ? s.x : (kind == 1 ? sqrtf(s.x) : pow_pos(s.x, a.alpha - 1.f));
-    const float step = s.x > 0.f ? (root - 1.f) * (s.x / root) / s.y : -INFINITY;
-    // half a unit in the last place of the scores that tau is compared with
-    const bool done = fabsf(step) <= 6e-8f * fmaxf(fabsf(tau), fabsf(top));
-    const float next = tau + step;
-    tau = next > lo && next < hi ? next : (done ? tau : 0.5f * (lo + hi));
-    if (done) break;
   }
 
-  // the support, in order: weight and key
-  int m = 0;
-  for (int i0 = 0; i0 < n; i0 += kFinThreads) {
-    const int i = i0 + tid;
-    uint2 e = make_uint2(0, 0);
-    float w = 0.f;
-    if (i < n) {
-      e = row.get(i);
-      w = entmax_weight(__uint_as_float(e.x), tau, kind, beta);
-    }
-    int all;
-    const int at = m + block_excl(w > 0.f, reinterpret_cast<int*>(scratch), &all);
-    if (w > 0.f) row.put(at, make_uint2(__float_as_uint(w), e.y));
-    m += all;
-  }
+  // ---- heavy rows: the whole block, one row after another
   __syncthreads();
-
-  float acc[EPL] = {};
-  const int sub = tid / LPR, col = tid % LPR * EPL;
-#pragma unroll 4
-  for (int i = sub; i < m; i += GROUPS) {
-    const uint2 e = row.get(i);
-    const float w = __uint_as_float(e.x);
-    const int key = (int)e.y;
-    const T* v;
-    bool ok = true;
-    if (key < 0) {
-      v = static_cast<const T*>(a.v_draft) + b * a.vs[0] + hkv * a.vs[1] + (int64_t)~key * a.vs[2];
+  for (int w = 0; w < kFinWarps; ++w) {
+    if (!s_heavy[w]) continue;                   // uniform over the block
+    __syncthreads();                             // the slots are free
+    r = fin_row(a, id0 + w, lane);
+    const float* const zd_w = reinterpret_cast<const float*>(s_dyn + n_ends) + w * a.tokens;
+    int all = 0;
+    float floor_w = -INFINITY;
+    if (a.dense) {
+      all = r.len;
+      if (w == warp && lane == 0) scratch[31] = floor_z;
+      __syncthreads();
+      floor_w = scratch[31];
     } else {
-      int page, in_page;
-      size_t off;
-      a.by_page.divmod(key, page, in_page);
-      ok = kv_page_offset(a.c, b, hkv, page, off);
-      v = static_cast<const T*>(a.c.v) + off + (size_t)in_page * D;
+      const int* const counts = a.counts + r.id * a.max_parts * a.sub;
+      const float* const bounds = a.bounds + r.id * a.max_parts * a.sub;
+      for (int i0 = 0; i0 < r.lists; i0 += kFinThreads) {
+        const bool in = i0 + tid < r.lists;
+        const int c = in ? counts[i0 + tid] : 0;
+        if (in) floor_w = fmaxf(floor_w, bounds[i0 + tid]);
+        int total;
+        const int before = block_excl(c, reinterpret_cast<int*>(scratch), &total);
+        if (in) s_dyn[i0 + tid] = all + before + c;
+        all += total;
+      }
+      floor_w = block_max(floor_w, scratch);
+      __syncthreads();
     }
-    float x[EPL];
-    unpack<T>(ok ? *reinterpret_cast<const uint4*>(v + col) : make_uint4(0, 0, 0, 0), x);
+    const int* const ends_w = s_dyn;
+    const FinHeavy rows{s_slots, r.region};
+    // what the largest bound leaves, in order; a NaN stays
+    n = 0;
+    top = -INFINITY;
+    for (int i0 = 0; i0 < all + a.tokens; i0 += kFinThreads) {
+      const int i = i0 + tid;
+      uint2 e = make_uint2(__float_as_uint(-INFINITY), 0);
+      if (i < all) e = fin_entry(a, r, ends_w, i);
+      else if (i < all + a.tokens) e = make_uint2(__float_as_uint(zd_w[i - all]), (uint32_t)~(i - all));
+      const bool keep = i < all + a.tokens && !(__uint_as_float(e.x) <= floor_w);
+      if (keep) top = max_nan(top, __uint_as_float(e.x));
+      int total;
+      const int at = n + block_excl(keep, reinterpret_cast<int*>(scratch), &total);
+      if (keep) rows.put(at, e);
+      n += total;
+    }
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) acc[j] = fmaf(w, x[j], acc[j]);
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    __syncthreads();
+    if (lane == 0) scratch[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kFinWarps; ++v) top = max_nan(top, scratch[v]);
+    if (!(fabsf(top) < INFINITY)) {
+      const float fill = top == -INFINITY ? 0.f : NAN;
+      if (tid < D) write(tid, fill);
+      if (tid == 0) write_tau(top == -INFINITY ? INFINITY : NAN);
+      continue;
+    }
+    const float tau = fin_tau(fmaxf(floor_w, top - 1.f), top, a.alpha, kind, [&](float t) {
+      float2 s = make_float2(0.f, 0.f);
+      float s2 = 0.f;
+      for (int i = tid; i < n; i += kFinThreads)
+        halley_accumulate(__uint_as_float(rows.get(i).x), t, kind, beta, s.x, s.y, s2);
+      return block_sum2(s, scratch);
+    });
+    int m = 0;
+    for (int i0 = 0; i0 < n; i0 += kFinThreads) {
+      const int i = i0 + tid;
+      uint2 e = make_uint2(0, 0);
+      float weight = 0.f;
+      if (i < n) {
+        e = rows.get(i);
+        weight = entmax_weight(__uint_as_float(e.x), tau, kind, beta);
+      }
+      int total;
+      const int at = m + block_excl(weight > 0.f, reinterpret_cast<int*>(scratch), &total);
+      if (weight > 0.f) rows.put(at, make_uint2(__float_as_uint(weight), e.y));
+      m += total;
+    }
+    __syncthreads();
+    float acc[EPL] = {};
+    const int sub = tid / LPR, col = tid % LPR * EPL;
+#pragma unroll 4
+    for (int i = sub; i < m; i += GROUPS) {
+      const uint2 e = rows.get(i);
+      float x[EPL];
+      unpack<T>(fin_value<T, D>(a, r, (int)e.y, col), x);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) acc[j] = fmaf(__uint_as_float(e.x), x[j], acc[j]);
+    }
+    __syncthreads();                             // the slots become partial sums
+    float* const s_acc = reinterpret_cast<float*>(s_slots);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) s_acc[sub * D + col + j] = acc[j];
+    __syncthreads();
+    if (tid < D) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) s += s_acc[i * D + tid];
+      write(tid, s);
+    }
+    if (tid == 0) write_tau(tau);
   }
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) s_acc[sub * D + col + j] = acc[j];
-  __syncthreads();
-  if (tid < D) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < GROUPS; ++i) s += s_acc[i * D + tid];
-    out[tid] = from_float<T>(s);
-  }
-  if (tid == 0 && tau_out) *tau_out = tau;
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 
 struct TreePlan {
   int64_t region;        // entries per row
-  int tiles, rows, sub, row_blocks, ranges, tile_keys;
+  int tiles, rows, sub, list_turn, list_cols, row_blocks, ranges, tile_keys;
   int64_t row_bytes;     // workspace per row
   int max_parts;
-  bool mma, sample;      // tensor cores; a sample before the pass
+  bool mma, dense;       // tensor cores; all scores written out, no sample
   int sample_tiles;
   TmShape shape;
 };
 
-constexpr int kSampleFrom = 8;         // tiles per block from which on there is a sample
+constexpr int kSampleFrom = 8;         // tiles per block from which on there is a sample (fewer: all scores)
 
 static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
   TreePlan p{};
   p.rows = tokens * (q_heads / c->kv_heads);
   p.mma = c->dtype != EKV_F32;
   p.tile_keys = kTreeTile;
+  p.list_turn = 1;
   if (p.mma) {
     TmShape& sh = p.shape;
-    const int blocks = (p.rows + kTmMaxRows - 1) / kTmMaxRows;
-    sh.n_rows = ((p.rows + blocks - 1) / blocks + 15) / 16 * 16;
-    p.row_blocks = (p.rows + sh.n_rows - 1) / sh.n_rows;
-    p.sub = kTmSub;
+    p.row_blocks = (p.rows + kTmMaxRows - 1) / kTmMaxRows;
+    sh.n_rows = (p.rows + p.row_blocks - 1) / p.row_blocks;
+    sh.row_tiles = sh.n_rows > kTreeTile ? 2 : 1;
+    sh.copies = sh.n_rows <= 32 ? 4 : (sh.n_rows <= 64 ? 2 : 1);
+    p.list_turn = sh.row_tiles == 2 ? 1 : 4;
+    p.list_cols = sh.row_tiles == 2 ? kTreeTile / 2 : kTreeTile / sh.copies;
+    p.sub = sh.row_tiles == 2 ? 2 : 4 * sh.copies;
     p.ranges = sm_count() / p.row_blocks;                 // one block per SM: its tiles fill the shared memory
-    for (sh.acc_cols = 16; sh.acc_cols < sh.n_rows;) sh.acc_cols *= 2;
-    for (sh.stages = kTmMaxStages; tm_smem_bytes(sh.n_rows, c->head_dim, sh.stages) > 227 * 1024;) --sh.stages;
+    for (sh.stages = kTmMaxStages; tm_smem_bytes(sh.row_tiles, c->head_dim, sh.stages) > 227 * 1024;) --sh.stages;
     // a copy must not cross a page: the largest divisor of the page size that fits a tile
     sh.box_rows = kTreeTile;
     if (c->block_table)
@@ -415,16 +587,17 @@ static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int 
   } else {
     p.row_blocks = (p.rows + kSimtRows - 1) / kSimtRows;
     p.sub = kSimtWarps;
+    p.list_cols = kTreeTile / kSimtWarps;
     p.ranges = 2 * sm_count() / p.row_blocks;
   }
   if (p.ranges < 1) p.ranges = 1;
   p.tiles = (int)(((int64_t)max_seq + p.tile_keys - 1) / p.tile_keys);
-  // drafted survivors are kept behind the cache's
-  p.region = (int64_t)p.tiles * kTreeTile + (tokens + 1) / 2 * 2;
   p.max_parts = p.ranges < p.tiles ? p.ranges : (p.tiles > 0 ? p.tiles : 1);
+  p.dense = p.mma && (int64_t)p.tiles * c->batch * c->kv_heads < (int64_t)kSampleFrom * p.ranges;
+  // drafted survivors are kept behind the cache's
+  p.region = ((int64_t)p.tiles + (p.dense ? 0 : (int64_t)p.max_parts * (p.list_turn - 1))) * kTreeTile + (tokens + 1) / 2 * 2;
   p.row_bytes = p.region * (int64_t)sizeof(uint2) + 8ll * p.max_parts * p.sub;
-  if (p.mma && (int64_t)p.tiles * c->batch * c->kv_heads >= (int64_t)kSampleFrom * p.ranges) {
-    p.sample = true;
+  if (p.mma && !p.dense) {
     p.sample_tiles = (p.tiles + kSampleStride - 1) / kSampleStride;
     if (p.sample_tiles > kSampleTiles) p.sample_tiles = kSampleTiles;
     p.row_bytes += 16ll * p.sample_tiles;
@@ -460,7 +633,7 @@ static int tree_k_map(CUtensorMap* map, const ekv_cache_desc* c, int box_rows) {
 }
 
 // what a launch may use of the GPU's memory before the groups are taken in several turns
-constexpr int64_t kTreeWorkspace = (int64_t)2 << 30;
+constexpr int64_t kTreeWorkspace = (int64_t)6 << 30;
 
 static int64_t tree_groups_per_turn(const TreePlan& p, int groups) {
   int64_t n = kTreeWorkspace / (p.row_bytes * p.rows);
@@ -471,13 +644,16 @@ template <typename T, int D>
 static int launch_scores(const TreeArgs& a, const TreePlan& p, const CUtensorMap& k_map, cudaStream_t st) {
   const unsigned grid = (unsigned)(a.ranges * a.row_blocks);
   if constexpr (sizeof(T) == 2) {
-    const int smem = (int)tm_smem_bytes(p.shape.n_rows, D, p.shape.stages);
-    const auto pass = tree_scores_mma_kernel<T, D, false>, sample = tree_scores_mma_kernel<T, D, true>;
-    cudaError_t e = cudaFuncSetAttribute(pass, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(sample, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
-    if (p.sample) sample<<<grid, kTmThreads, smem, st>>>(a, k_map, p.shape);
-    pass<<<grid, kTmThreads, smem, st>>>(a, k_map, p.shape);
+    const int smem = (int)tm_smem_bytes(p.shape.row_tiles, D, p.shape.stages);
+    const auto run = [&](auto kernel) -> int {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return (int)e;
+      kernel<<<grid, kTmThreads, smem, st>>>(a, k_map, p.shape);
+      return EKV_OK;
+    };
+    if (p.dense) return run(tree_scores_mma_kernel<T, D, TM_DENSE>);
+    if (int e = run(tree_scores_mma_kernel<T, D, TM_SAMPLE>)) return e;
+    return run(tree_scores_mma_kernel<T, D, TM_LISTS>);
   } else {
     const size_t smem = sizeof(float) * (kSimtRows + kSimtKeys) * (D + 4);
     cudaError_t e = cudaFuncSetAttribute(tree_scores_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -563,10 +739,13 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   a.counts = reinterpret_cast<int*>(a.entries + turn * p.rows * p.region);
   a.bounds = reinterpret_cast<float*>(a.counts + turn * p.rows * p.max_parts * p.sub);
   a.classes = a.bounds + turn * p.rows * p.max_parts * p.sub;
-  a.sample = p.sample;
+  a.dense = p.dense;
+  a.list_turn = p.list_turn;
+  a.list_cols = p.list_cols;
   a.sample_tiles = p.sample_tiles;
   a.tile_keys = p.tile_keys;
-  const size_t fin_smem = sizeof(int) * ((size_t)p.max_parts * p.sub + 1 + tokens);
+  const int n_ends = fin_ends(p.max_parts * p.sub);
+  const size_t fin_smem = sizeof(int) * ((size_t)n_ends + (size_t)kFinWarps * tokens);
   cudaStream_t st = as_stream(stream);
   CUtensorMap k_map{};
   if (p.mma && max_seq_len > 0)
@@ -580,7 +759,13 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
     EKV_DISPATCH(c->dtype, c->head_dim, {
       if (max_seq_len > 0) err = launch_scores<T, D>(a, p, k_map, st);
       if (err) return err;
-      tree_finish_kernel<T, D><<<(unsigned)rows, kFinThreads, fin_smem, st>>>(a);
+      if (fin_smem > 12 * 1024) {                         // beside the kernel's own 33 KB
+        cudaError_t e = cudaFuncSetAttribute(tree_finish_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)fin_smem);
+        if (e != cudaSuccess) return (int)e;
+      }
+      tree_finish_kernel<T, D><<<(unsigned)((rows + kFinWarps - 1) / kFinWarps), kFinThreads, fin_smem, st>>>(a, rows,
+                                                                                                              n_ends);
     });
   }
   return launch_status();

@@ -5,7 +5,7 @@
 // sum (z - tau)_+^beta v.  The tau of some of the keys is a lower bound of the tau of all of them, and a key below a
 // lower bound has no weight.  Three kernels:
 //
-//   sample   (long sequences) scores a few tiles of every sequence and keeps each row's largest scores of disjoint
+//   sample   (not for few keys) scores a few tiles of every sequence and keeps each row's largest scores of disjoint
 //            classes of keys; their tau is the row's bound.
 //   scores   one pass over K.  The rows that share a KV head are scored together, and each row keeps a list of the
 //            (z, key) above its bound.
@@ -22,7 +22,7 @@
 namespace ekv {
 
 constexpr int kTreeTile = 128;         // places for keys in a tile
-constexpr int kSampleTiles = 64;       // tiles of a sequence in its sample, at most
+constexpr int kSampleTiles = 128;       // tiles of a sequence in its sample, at most
 constexpr int kSampleStride = 8;       // and at most every eighth one
 
 struct TreeArgs {
@@ -44,16 +44,17 @@ struct TreeArgs {
   int max_seq;                         // lengths are clipped to this (the row regions' size)
   // one launch covers the (sequence, KV head) groups [g0, g1) and the rows [row0, row0 + rows) of each; row = t * group + g
   int g0, g1, row0, rows;
-  int ranges, row_blocks, sub;         // pieces of the tile sequence; row blocks; lists per row and piece
+  int ranges, row_blocks;              // pieces of the tile sequence; row blocks
+  int sub, list_turn, list_cols;       // lists per row and piece, each of list_cols columns of every list_turn-th tile
+  int dense;                           // no lists: all scores of a row, floats from the middle of its region
   int max_parts;                       // pieces of one group, at most
   uint2* entries;                      // [groups][rows][region]: z bits, key
   int64_t region;
   int* counts;                         // [groups][rows][max_parts * sub]
   float* bounds;                       // same shape: tau lies above, and the list misses no key of its share that does
   int tile_keys;                       // keys of a tile (kTreeTile, or less: whole boxes of the copies)
-  int sample;                          // there is a sample
-  int sample_tiles;                    // tiles of one group in it, at most
-  float* classes;                      // [groups][rows][sample_tiles][4]: largest raw score of a lane quadrant
+  int sample_tiles;                    // tiles of one group in the sample, at most
+  float* classes;                      // [groups][rows][sample_tiles][4]: largest raw score of 32 keys
   int* status;
 };
 
@@ -81,55 +82,6 @@ __device__ __forceinline__ int tree_drafts(const TreeArgs& a, int b) {
   return a.draft_lens ? min(max(a.draft_lens[b], 0), a.tokens) : a.tokens;
 }
 
-// Tiles of the launch's groups before group g (warp-cooperative; every lane gets the sum).
-template <bool SAMPLE = false>
-__device__ __forceinline__ int64_t tree_tiles_before(const TreeArgs& a, int g, int lane) {
-  const int H = a.c.kv_heads;
-  const int b0 = a.g0 / H, b1 = g / H;
-  int64_t n = 0;
-  for (int b = b0 + lane; b <= b1 && b < a.c.batch; b += 32) {
-    const int lo = max(a.g0, b * H), hi = min(g, (b + 1) * H);
-    n += (int64_t)(hi - lo) * tree_tiles<SAMPLE>(a, b);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
-}
-
-// The group that tile `t` of the launch's tile sequence lies in, and that group's first tile (warp-cooperative; t must
-// lie in the sequence).
-struct TreeAt {
-  int g;
-  int64_t first;
-};
-template <bool SAMPLE = false>
-__device__ __forceinline__ TreeAt tree_find(const TreeArgs& a, int64_t t, int lane) {
-  const int H = a.c.kv_heads;
-  int64_t before = 0;
-  for (int b0 = a.g0 / H; b0 < a.c.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const int lo = max(a.g0, b * H), hi = min(a.g1, (b + 1) * H);
-    const int per = b < a.c.batch && hi > lo ? tree_tiles<SAMPLE>(a, b) : 0;
-    int64_t end = (int64_t)max(hi - lo, 0) * per;
-    const int64_t mine = end;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t n = __shfl_up_sync(0xffffffffu, end, o);
-      if (lane >= o) end += n;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + end > t);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int64_t start = before + __shfl_sync(0xffffffffu, end - mine, src);
-      const int tiles = __shfl_sync(0xffffffffu, per, src), first = __shfl_sync(0xffffffffu, lo, src);
-      const int64_t skip = (t - start) / tiles;
-      return TreeAt{first + (int)skip, start + skip * tiles};
-    }
-    before += __shfl_sync(0xffffffffu, end, 31);
-  }
-  return TreeAt{a.g1, before};
-}
-
 // The tile sequence of W tiles in N pieces (N <= W): piece i is [i W / N, (i + 1) W / N).
 struct TreeSplit {
   int64_t W;
@@ -137,11 +89,99 @@ struct TreeSplit {
   __device__ __forceinline__ int64_t begin(int i) const { return i * W / N; }
   __device__ __forceinline__ int piece_of(int64_t tile) const { return (int)(((tile + 1) * N - 1) / W); }
 };
-__device__ __forceinline__ TreeSplit tree_split(int64_t W, int ranges) {
-  TreeSplit s;
-  s.W = W;
-  s.N = (int)min((int64_t)ranges, W);
-  return s;
+
+// The lengths of 32 sequences at a time, one per lane: tiles of this lane's sequence that belong to the launch, and the
+// launch's groups among its KV heads.
+struct TreeLane {
+  int first, tiles;      // first group, tiles per group
+  int64_t all, end;      // tiles of this sequence; running sum with it
+};
+template <bool SAMPLE>
+__device__ __forceinline__ TreeLane tree_lane(const TreeArgs& a, int b0, int lane, int64_t before) {
+  const int H = a.c.kv_heads, b = b0 + lane;
+  TreeLane t;
+  t.first = max(a.g0, b * H);
+  const int groups = max(min(a.g1, (b + 1) * H) - t.first, 0);
+  t.tiles = b < a.c.batch && groups > 0 ? tree_tiles<SAMPLE>(a, b) : 0;
+  t.all = t.end = (int64_t)groups * t.tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t n = __shfl_up_sync(0xffffffffu, t.end, o);
+    if (lane >= o) t.end += n;
+  }
+  t.end += before;
+  return t;
+}
+
+// Warp-cooperative: what piece `range` of the launch's tile sequence covers, and the group that it begins in.  An empty
+// piece has t_begin == t_end.
+struct TreeRange {
+  TreeSplit split;
+  int64_t t_begin, t_end;
+  int g;
+  int64_t first;         // the group's first tile
+};
+template <bool SAMPLE>
+__device__ __forceinline__ TreeRange tree_range(const TreeArgs& a, int range, int lane) {
+  const int b_first = a.g0 / a.c.kv_heads, b_last = (a.g1 - 1) / a.c.kv_heads;
+  TreeRange r;
+  int64_t W = 0;
+  TreeLane t;
+  for (int b0 = b_first; b0 <= b_last; b0 += 32) {
+    t = tree_lane<SAMPLE>(a, b0, lane, W);
+    W = __shfl_sync(0xffffffffu, t.end, 31);
+  }
+  r.split.W = W;
+  r.split.N = (int)min((int64_t)a.ranges, W);
+  r.t_begin = r.t_end = 0;
+  r.g = a.g1;
+  r.first = 0;
+  if (W == 0 || range >= r.split.N) return r;
+  r.t_begin = r.split.begin(range);
+  r.t_end = r.split.begin(range + 1);
+  int64_t before = 0;
+  for (int b0 = b_first; b0 <= b_last; b0 += 32) {
+    if (b_last - b_first >= 32) t = tree_lane<SAMPLE>(a, b0, lane, before);     // else it is still in the registers
+    const unsigned hit = __ballot_sync(0xffffffffu, t.end > r.t_begin);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int64_t start = __shfl_sync(0xffffffffu, t.end - t.all, src);
+      const int64_t skip = (r.t_begin - start) / __shfl_sync(0xffffffffu, t.tiles, src);
+      r.g = __shfl_sync(0xffffffffu, t.first, src) + (int)skip;
+      r.first = start + skip * __shfl_sync(0xffffffffu, t.tiles, src);
+      break;
+    }
+    before = __shfl_sync(0xffffffffu, t.end, 31);
+  }
+  return r;
+}
+
+// Warp-cooperative: the launch's split, and the first tile of group g.
+struct TreeGroup {
+  TreeSplit split;
+  int64_t first;
+};
+__device__ __forceinline__ TreeGroup tree_group(const TreeArgs& a, int g, int lane) {
+  const int H = a.c.kv_heads, b_first = a.g0 / H, b_last = (a.g1 - 1) / H, b = g / H;
+  TreeGroup r;
+  int64_t W = 0;
+  r.first = 0;
+  for (int b0 = b_first; b0 <= b_last; b0 += 32) {
+    const TreeLane t = tree_lane<false>(a, b0, lane, W);
+    if (b >= b0 && b < b0 + 32)
+      r.first = __shfl_sync(0xffffffffu, t.end - t.all, b - b0) +
+                (int64_t)(g - __shfl_sync(0xffffffffu, t.first, b - b0)) * __shfl_sync(0xffffffffu, t.tiles, b - b0);
+    W = __shfl_sync(0xffffffffu, t.end, 31);
+  }
+  r.split.W = W;
+  r.split.N = (int)min((int64_t)a.ranges, W);
+  return r;
+}
+
+// Where list s of a row's part begins in the row's region: the part-th piece of the group, `tiles` tiles from `tile0`.
+__device__ __forceinline__ int64_t tree_list_place(const TreeArgs& a, int64_t tile0, int part, int64_t tiles, int s) {
+  return (tile0 + (int64_t)part * (a.list_turn - 1)) * kTreeTile +
+         s * ((tiles + a.list_turn - 1) / a.list_turn) * a.list_cols;
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) {      // a NaN stays
