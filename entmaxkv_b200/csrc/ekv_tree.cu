@@ -24,14 +24,14 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
   const int H = a.c.kv_heads;
   const TreeRange at = tree_range<false>(a, range, lane);
   if (at.t_begin == at.t_end) return;
-  const int64_t t_begin = at.t_begin, t_end = at.t_end;
-  int64_t g_first = at.first;                           // first tile of the group
+  const int t_begin = at.t_begin, t_end = at.t_end;
+  int g_first = at.first;                           // first tile of the group
   for (int g = at.g; g < a.g1 && g_first < t_end; ++g) {
     const int b = g / H, hkv = g % H;
     const int n = tree_tiles(a, b);
     if (n == 0) continue;
-    const int64_t g_end = g_first + n;
-    const int tile0 = (int)(max(t_begin, g_first) - g_first), tile1 = (int)(min(t_end, g_end) - g_first);
+    const int g_end = g_first + n;
+    const int tile0 = max(t_begin, g_first) - g_first, tile1 = min(t_end, g_end) - g_first;
     const int part = range - at.split.piece_of(g_first);
     const int len = tree_len(a, b);
     const int live = min(tree_drafts(a, b) * a.group - a.row0, a.rows) - rb * kSimtRows;   // rows of this block
@@ -106,19 +106,13 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
   }
 }
 
-__device__ __forceinline__ float warp_max_nan(float v) {
-  float r;
-  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // ---- tau and output ------------------------------------------------------------------------------------------------
 //
-// A warp per row while at most 512 candidates lie above the row's best bound (the usual case: no barrier, sums by
+// A warp per row while at most 1024 candidates lie above the row's best bound (the usual case: no barrier, sums by
 // shuffle), the whole block per row where more do (flat scores), one such row after another.
 
 constexpr int kFinThreads = 256, kFinWarps = kFinThreads / 32;
-constexpr int kFinLight = 512;                  // survivors of a row that one warp finishes
+constexpr int kFinLight = 1024;                 // survivors of a row that one warp finishes
 constexpr int kFinLists = 256;                  // and its lists
 constexpr int kFinSlots = kFinWarps * kFinLight;   // of a heavy row on chip; more stay in the row's region
 
@@ -126,7 +120,7 @@ constexpr int kFinSlots = kFinWarps * kFinLight;   // of a heavy row on chip; mo
 struct FinRow {
   int b, hkv, hq, t, drafts;
   int64_t id;
-  int64_t first;                                // the group's first tile
+  int first;                                    // the group's first tile
   int tiles, piece0, lists, len;
   TreeSplit split;
   uint2* region;
@@ -152,18 +146,22 @@ __device__ __forceinline__ FinRow fin_row(const TreeArgs& a, int64_t id, int lan
   r.lists = r.tiles ? (r.split.piece_of(r.first + r.tiles - 1) - r.piece0 + 1) * a.sub : 0;
   return r;
 }
-// entry i of the concatenation of the row's lists, which end at ends[] (or of all its scores)
-__device__ __forceinline__ uint2 fin_entry(const TreeArgs& a, const FinRow& r, const int* ends, int i) {
+// A list of a row: its end in their concatenation, and what leads from a place in that to one in the row's region.
+__device__ __forceinline__ int2 fin_list(const TreeArgs& a, const FinRow& r, int l, int before, int count) {
+  const int p = l / a.sub, s = l % a.sub;
+  const int t0 = max(r.split.begin(r.piece0 + p), r.first) - r.first;
+  const int t1 = min(r.split.begin(r.piece0 + p + 1), r.first + r.tiles) - r.first;
+  return make_int2(before + count, tree_list_place(a, t0, p, t1 - t0, s) - before);
+}
+// entry i of the concatenation of the row's lists (or of all its scores)
+__device__ __forceinline__ uint2 fin_entry(const TreeArgs& a, const FinRow& r, const int2* lists, int i) {
   if (a.dense) return make_uint2(__float_as_uint(reinterpret_cast<const float*>(r.region)[a.region + i]), (uint32_t)i);
   int lo = 0, hi = r.lists - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (ends[mid] > i) hi = mid; else lo = mid + 1;
+    if (lists[mid].x > i) hi = mid; else lo = mid + 1;
   }
-  const int p = lo / a.sub, s = lo % a.sub;
-  const int64_t t0 = max(r.split.begin(r.piece0 + p), r.first) - r.first;
-  const int64_t t1 = min(r.split.begin(r.piece0 + p + 1), r.first + r.tiles) - r.first;
-  return r.region[tree_list_place(a, t0, p, t1 - t0, s) + (i - (lo ? ends[lo - 1] : 0))];
+  return r.region[lists[lo].y + i];
 }
 // 16 bytes of the value row of a key (or, ~j, of a drafted token)
 template <typename T, int D>
@@ -273,28 +271,29 @@ struct FinHeavy {
   __device__ __forceinline__ void put(int i, uint2 e) const { (i < kFinSlots ? slots[i] : region[i]) = e; }
 };
 
-// list ends in shared memory: kFinLists per warp, or all lists of one row
+// lists in shared memory: kFinLists per warp, or all of one row
 static inline int fin_ends(int max_lists) {
   const int each = max_lists < kFinLists ? max_lists : kFinLists;
   return each * kFinWarps > max_lists ? each * kFinWarps : max_lists;
 }
 
-// dynamic shared memory: [n_ends] list ends, [warps][tokens] drafted scores
+// dynamic shared memory: [n_ends] lists, [warps][tokens] drafted scores
 template <typename T, int D>
 __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __grid_constant__ TreeArgs a, const int64_t n_rows,
                                                                      const int n_ends) {
   constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL, SIDE = 32 / LPR, GROUPS = kFinThreads / LPR;
-  __shared__ uint2 s_slots[kFinSlots];
   __shared__ float scratch[32];
   __shared__ int s_heavy[kFinWarps];
-  extern __shared__ int s_dyn[];
+  extern __shared__ uint2 s_slots[];                   // [kFinSlots], then the lists
+  int2* const s_dyn = reinterpret_cast<int2*>(s_slots + kFinSlots);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int* const ends = s_dyn + warp * min(a.max_parts * a.sub, kFinLists);
+  int2* const lists = s_dyn + warp * min(a.max_parts * a.sub, kFinLists);
   float* const zd = reinterpret_cast<float*>(s_dyn + n_ends) + warp * a.tokens;
   const int64_t id0 = (int64_t)blockIdx.x * kFinWarps;
   const int kind = alpha_kind_of(a.alpha);
   const float beta = 1.f / (a.alpha - 1.f);
 
+  tree_wait_for_previous();
   FinRow r{};
   bool mine = id0 + warp < n_rows, heavy = false;
   if (mine) {
@@ -313,53 +312,58 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
       const float* const bounds = a.bounds + r.id * a.max_parts * a.sub;
       for (int i0 = 0; i0 < r.lists; i0 += 32) {
         const bool in = i0 + lane < r.lists;
-        int end = in ? counts[i0 + lane] : 0;
+        const int c = in ? counts[i0 + lane] : 0;
+        int end = c;
         if (in) floor_z = fmaxf(floor_z, bounds[i0 + lane]);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int m = __shfl_up_sync(0xffffffffu, end, o);
           if (lane >= o) end += m;
         }
-        if (in) ends[i0 + lane] = raw + end;
+        if (in) lists[i0 + lane] = fin_list(a, r, i0 + lane, raw + end - c, c);
         raw += __shfl_sync(0xffffffffu, end, 31);
       }
       floor_z = warp_max(floor_z);
     }
     fin_drafts<T, D>(a, r, zd, lane / LPR, SIDE, lane);
     __syncwarp();
-    if (a.dense) {                               // nothing bounds tau yet: the maximum first
-      const float* const z = reinterpret_cast<const float*>(r.region) + a.region;
-#pragma unroll 8
-      for (int i = lane; i < raw; i += 32) top = max_nan(top, z[i]);
-      for (int j = lane; j < a.tokens; j += 32) top = max_nan(top, zd[j]);
-      top = warp_max_nan(top);
-      floor_z = top - 1.f;
-    }
-    // what lies above the floor, in order; a NaN stays
-    constexpr int AT_ONCE = 4;
+    // what lies above the floor, in order; a NaN stays.  The floor follows the maximum, and where too much was kept under
+    // an early one, the slots are gone through again
+    constexpr int AT_ONCE = 8;
     for (int i0 = 0; i0 < raw + a.tokens && n <= kFinLight; i0 += 32 * AT_ONCE) {
       uint2 e[AT_ONCE];
+      float most = -INFINITY;
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
         const int i = i0 + 32 * k + lane;
         e[k] = make_uint2(__float_as_uint(-INFINITY), 0);
-        if (i < raw) e[k] = fin_entry(a, r, ends, i);
+        if (i < raw) e[k] = fin_entry(a, r, lists, i);
         else if (i < raw + a.tokens) e[k] = make_uint2(__float_as_uint(zd[i - raw]), (uint32_t)~(i - raw));   // ~j: drafted
+        most = max_nan(most, __uint_as_float(e[k].x));
+      }
+      top = max_nan(top, warp_max_nan(most));
+      floor_z = fmaxf(floor_z, top - 1.f);
+      if (n > kFinLight - 32 * AT_ONCE) {
+        int kept = 0;
+        for (int j0 = 0; j0 < n; j0 += 32) {
+          const uint2 x = j0 + lane < n ? slots[j0 + lane] : make_uint2(__float_as_uint(-INFINITY), 0);
+          const bool keep = !(__uint_as_float(x.x) <= floor_z);
+          const unsigned has = __ballot_sync(0xffffffffu, keep);
+          if (keep) slots[kept + __popc(has & ((1u << lane) - 1))] = x;
+          kept += __popc(has);
+          __syncwarp();
+        }
+        n = kept;
       }
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
-        const float z = __uint_as_float(e[k].x);
-        const bool keep = !(z <= floor_z);
+        const bool keep = !(__uint_as_float(e[k].x) <= floor_z);
         const unsigned has = __ballot_sync(0xffffffffu, keep);
         const int to = n + __popc(has & ((1u << lane) - 1));
-        if (keep) {
-          top = max_nan(top, z);
-          if (to < kFinLight) slots[to] = e[k];
-        }
+        if (keep && to < kFinLight) slots[to] = e[k];
         n += __popc(has);
       }
     }
-    top = warp_max_nan(top);
     heavy = n > kFinLight;
     __syncwarp();
   }
@@ -451,11 +455,18 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
     const float* const zd_w = reinterpret_cast<const float*>(s_dyn + n_ends) + w * a.tokens;
     int all = 0;
     float floor_w = -INFINITY;
-    if (a.dense) {
+    if (a.dense) {                               // nothing bounds tau yet: the maximum first
       all = r.len;
-      if (w == warp && lane == 0) scratch[31] = floor_z;
+      const float* const z = reinterpret_cast<const float*>(r.region) + a.region;
+      for (int i = tid; i < all; i += kFinThreads) floor_w = max_nan(floor_w, z[i]);
+      for (int j = tid; j < a.tokens; j += kFinThreads) floor_w = max_nan(floor_w, zd_w[j]);
+      floor_w = warp_max_nan(floor_w);
+      if (lane == 0) scratch[warp] = floor_w;
       __syncthreads();
-      floor_w = scratch[31];
+#pragma unroll
+      for (int v = 0; v < kFinWarps; ++v) floor_w = max_nan(floor_w, scratch[v]);
+      floor_w -= 1.f;
+      __syncthreads();
     } else {
       const int* const counts = a.counts + r.id * a.max_parts * a.sub;
       const float* const bounds = a.bounds + r.id * a.max_parts * a.sub;
@@ -465,13 +476,12 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
         if (in) floor_w = fmaxf(floor_w, bounds[i0 + tid]);
         int total;
         const int before = block_excl(c, reinterpret_cast<int*>(scratch), &total);
-        if (in) s_dyn[i0 + tid] = all + before + c;
+        if (in) s_dyn[i0 + tid] = fin_list(a, r, i0 + tid, all + before, c);
         all += total;
       }
       floor_w = block_max(floor_w, scratch);
       __syncthreads();
     }
-    const int* const ends_w = s_dyn;
     const FinHeavy rows{s_slots, r.region};
     // what the largest bound leaves, in order; a NaN stays
     n = 0;
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
     for (int i0 = 0; i0 < all + a.tokens; i0 += kFinThreads) {
       const int i = i0 + tid;
       uint2 e = make_uint2(__float_as_uint(-INFINITY), 0);
-      if (i < all) e = fin_entry(a, r, ends_w, i);
+      if (i < all) e = fin_entry(a, r, s_dyn, i);
       else if (i < all + a.tokens) e = make_uint2(__float_as_uint(zd_w[i - all]), (uint32_t)~(i - all));
       const bool keep = i < all + a.tokens && !(__uint_as_float(e.x) <= floor_w);
       if (keep) top = max_nan(top, __uint_as_float(e.x));
@@ -562,6 +572,8 @@ struct TreePlan {
 
 constexpr int kSampleFrom = 8;         // tiles per block from which on there is a sample (fewer: all scores)
 
+constexpr int kDenseTiles = 64;        // and tiles per sequence up to which that holds
+
 static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
   TreePlan p{};
   p.rows = tokens * (q_heads / c->kv_heads);
@@ -593,14 +605,14 @@ static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int 
   if (p.ranges < 1) p.ranges = 1;
   p.tiles = (int)(((int64_t)max_seq + p.tile_keys - 1) / p.tile_keys);
   p.max_parts = p.ranges < p.tiles ? p.ranges : (p.tiles > 0 ? p.tiles : 1);
-  p.dense = p.mma && (int64_t)p.tiles * c->batch * c->kv_heads < (int64_t)kSampleFrom * p.ranges;
+  p.dense = p.mma && p.tiles <= kDenseTiles && (int64_t)p.tiles * c->batch * c->kv_heads < (int64_t)kSampleFrom * p.ranges;
   // drafted survivors are kept behind the cache's
   p.region = ((int64_t)p.tiles + (p.dense ? 0 : (int64_t)p.max_parts * (p.list_turn - 1))) * kTreeTile + (tokens + 1) / 2 * 2;
   p.row_bytes = p.region * (int64_t)sizeof(uint2) + 8ll * p.max_parts * p.sub;
   if (p.mma && !p.dense) {
     p.sample_tiles = (p.tiles + kSampleStride - 1) / kSampleStride;
     if (p.sample_tiles > kSampleTiles) p.sample_tiles = kSampleTiles;
-    p.row_bytes += 16ll * p.sample_tiles;
+    p.row_bytes += 16ll * p.sample_tiles + 4;
   }
   return p;
 }
@@ -637,7 +649,25 @@ constexpr int64_t kTreeWorkspace = (int64_t)6 << 30;
 
 static int64_t tree_groups_per_turn(const TreePlan& p, int groups) {
   int64_t n = kTreeWorkspace / (p.row_bytes * p.rows);
+  if (p.tiles > 0 && n > kTreeMaxTiles / p.tiles) n = kTreeMaxTiles / p.tiles;
   return n < 1 ? 1 : (n > groups ? groups : n);
+}
+
+// `after`: the kernel may start while the one before it in the stream still runs (it waits itself before it uses results)
+template <typename... P, typename... V>
+static cudaError_t launch_after(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t st, bool after,
+                                const V&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = after ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename T, int D>
@@ -645,15 +675,17 @@ static int launch_scores(const TreeArgs& a, const TreePlan& p, const CUtensorMap
   const unsigned grid = (unsigned)(a.ranges * a.row_blocks);
   if constexpr (sizeof(T) == 2) {
     const int smem = (int)tm_smem_bytes(p.shape.row_tiles, D, p.shape.stages);
-    const auto run = [&](auto kernel) -> int {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (e != cudaSuccess) return (int)e;
-      kernel<<<grid, kTmThreads, smem, st>>>(a, k_map, p.shape);
-      return EKV_OK;
+    const auto run = [&](auto kernel, bool after) -> int {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e == cudaSuccess) e = launch_after(kernel, grid, kTmThreads, smem, st, after, a, k_map, p.shape);
+      return (int)e;
     };
-    if (p.dense) return run(tree_scores_mma_kernel<T, D, TM_DENSE>);
-    if (int e = run(tree_scores_mma_kernel<T, D, TM_SAMPLE>)) return e;
-    return run(tree_scores_mma_kernel<T, D, TM_LISTS>);
+    if (p.dense) return run(tree_scores_mma_kernel<T, D, TM_DENSE>, false);
+    if (int e = run(tree_scores_mma_kernel<T, D, TM_SAMPLE>, false)) return e;
+    const int64_t rows = (int64_t)(a.g1 - a.g0) * p.rows;
+    const cudaError_t e = launch_after(tree_bounds_kernel, (unsigned)((rows + 7) / 8), 256, 0, st, true, a, rows);
+    if (e != cudaSuccess) return (int)e;
+    return run(tree_scores_mma_kernel<T, D, TM_LISTS>, true);
   } else {
     const size_t smem = sizeof(float) * (kSimtRows + kSimtKeys) * (D + 4);
     cudaError_t e = cudaFuncSetAttribute(tree_scores_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -739,13 +771,14 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   a.counts = reinterpret_cast<int*>(a.entries + turn * p.rows * p.region);
   a.bounds = reinterpret_cast<float*>(a.counts + turn * p.rows * p.max_parts * p.sub);
   a.classes = a.bounds + turn * p.rows * p.max_parts * p.sub;
+  a.row_bounds = a.classes + turn * p.rows * p.sample_tiles * 4;
   a.dense = p.dense;
   a.list_turn = p.list_turn;
   a.list_cols = p.list_cols;
   a.sample_tiles = p.sample_tiles;
   a.tile_keys = p.tile_keys;
   const int n_ends = fin_ends(p.max_parts * p.sub);
-  const size_t fin_smem = sizeof(int) * ((size_t)n_ends + (size_t)kFinWarps * tokens);
+  const size_t fin_smem = sizeof(uint2) * ((size_t)kFinSlots + n_ends) + sizeof(float) * (size_t)kFinWarps * tokens;
   cudaStream_t st = as_stream(stream);
   CUtensorMap k_map{};
   if (p.mma && max_seq_len > 0)
@@ -759,13 +792,12 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
     EKV_DISPATCH(c->dtype, c->head_dim, {
       if (max_seq_len > 0) err = launch_scores<T, D>(a, p, k_map, st);
       if (err) return err;
-      if (fin_smem > 12 * 1024) {                         // beside the kernel's own 33 KB
-        cudaError_t e = cudaFuncSetAttribute(tree_finish_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)fin_smem);
-        if (e != cudaSuccess) return (int)e;
-      }
-      tree_finish_kernel<T, D><<<(unsigned)((rows + kFinWarps - 1) / kFinWarps), kFinThreads, fin_smem, st>>>(a, rows,
-                                                                                                              n_ends);
+      cudaError_t e = cudaFuncSetAttribute(tree_finish_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)fin_smem);
+      if (e == cudaSuccess)
+        e = launch_after(tree_finish_kernel<T, D>, (unsigned)((rows + kFinWarps - 1) / kFinWarps), kFinThreads, fin_smem,
+                         st, max_seq_len > 0, a, rows, n_ends);
+      if (e != cudaSuccess) return (int)e;
     });
   }
   return launch_status();

@@ -6,7 +6,7 @@
 // lower bound has no weight.  Three kernels:
 //
 //   sample   (not for few keys) scores a few tiles of every sequence and keeps each row's largest scores of disjoint
-//            classes of keys; their tau is the row's bound.
+//            classes of keys; a small kernel makes their tau the row's bound.
 //   scores   one pass over K.  The rows that share a KV head are scored together, and each row keeps a list of the
 //            (z, key) above its bound.
 //   finish   one block per row: adds the drafted keys, solves tau on the lists and sums the value rows of the support.
@@ -24,6 +24,7 @@ namespace ekv {
 constexpr int kTreeTile = 128;         // places for keys in a tile
 constexpr int kSampleTiles = 128;       // tiles of a sequence in its sample, at most
 constexpr int kSampleStride = 8;       // and at most every eighth one
+constexpr int kTreeMaxTiles = 1 << 23; // tiles of a launch, with at most 512 pieces
 
 struct TreeArgs {
   ekv_cache_desc c;
@@ -55,6 +56,7 @@ struct TreeArgs {
   int tile_keys;                       // keys of a tile (kTreeTile, or less: whole boxes of the copies)
   int sample_tiles;                    // tiles of one group in the sample, at most
   float* classes;                      // [groups][rows][sample_tiles][4]: largest raw score of 32 keys
+  float* row_bounds;                   // [groups][rows]: the sample's bound of tau, in raw score units
   int* status;
 };
 
@@ -82,31 +84,30 @@ __device__ __forceinline__ int tree_drafts(const TreeArgs& a, int b) {
   return a.draft_lens ? min(max(a.draft_lens[b], 0), a.tokens) : a.tokens;
 }
 
-// The tile sequence of W tiles in N pieces (N <= W): piece i is [i W / N, (i + 1) W / N).
+// The tile sequence of W tiles in N pieces (N <= W): piece i is [i W / N, (i + 1) W / N).  W N < 2^32 (see kTreeMaxTiles).
 struct TreeSplit {
-  int64_t W;
-  int N;
-  __device__ __forceinline__ int64_t begin(int i) const { return i * W / N; }
-  __device__ __forceinline__ int piece_of(int64_t tile) const { return (int)(((tile + 1) * N - 1) / W); }
+  unsigned W, N;
+  __device__ __forceinline__ int begin(int i) const { return (int)((unsigned)i * W / N); }
+  __device__ __forceinline__ int piece_of(int tile) const { return (int)((((unsigned)tile + 1) * N - 1) / W); }
 };
 
 // The lengths of 32 sequences at a time, one per lane: tiles of this lane's sequence that belong to the launch, and the
 // launch's groups among its KV heads.
 struct TreeLane {
   int first, tiles;      // first group, tiles per group
-  int64_t all, end;      // tiles of this sequence; running sum with it
+  int all, end;          // tiles of this sequence; running sum with it
 };
 template <bool SAMPLE>
-__device__ __forceinline__ TreeLane tree_lane(const TreeArgs& a, int b0, int lane, int64_t before) {
+__device__ __forceinline__ TreeLane tree_lane(const TreeArgs& a, int b0, int lane, int before) {
   const int H = a.c.kv_heads, b = b0 + lane;
   TreeLane t;
   t.first = max(a.g0, b * H);
   const int groups = max(min(a.g1, (b + 1) * H) - t.first, 0);
   t.tiles = b < a.c.batch && groups > 0 ? tree_tiles<SAMPLE>(a, b) : 0;
-  t.all = t.end = (int64_t)groups * t.tiles;
+  t.all = t.end = groups * t.tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t n = __shfl_up_sync(0xffffffffu, t.end, o);
+    const int n = __shfl_up_sync(0xffffffffu, t.end, o);
     if (lane >= o) t.end += n;
   }
   t.end += before;
@@ -117,37 +118,37 @@ __device__ __forceinline__ TreeLane tree_lane(const TreeArgs& a, int b0, int lan
 // piece has t_begin == t_end.
 struct TreeRange {
   TreeSplit split;
-  int64_t t_begin, t_end;
+  int t_begin, t_end;
   int g;
-  int64_t first;         // the group's first tile
+  int first;             // the group's first tile
 };
 template <bool SAMPLE>
 __device__ __forceinline__ TreeRange tree_range(const TreeArgs& a, int range, int lane) {
   const int b_first = a.g0 / a.c.kv_heads, b_last = (a.g1 - 1) / a.c.kv_heads;
   TreeRange r;
-  int64_t W = 0;
+  int W = 0;
   TreeLane t;
   for (int b0 = b_first; b0 <= b_last; b0 += 32) {
     t = tree_lane<SAMPLE>(a, b0, lane, W);
     W = __shfl_sync(0xffffffffu, t.end, 31);
   }
   r.split.W = W;
-  r.split.N = (int)min((int64_t)a.ranges, W);
+  r.split.N = min(a.ranges, W);
   r.t_begin = r.t_end = 0;
   r.g = a.g1;
   r.first = 0;
-  if (W == 0 || range >= r.split.N) return r;
+  if (W == 0 || range >= (int)r.split.N) return r;
   r.t_begin = r.split.begin(range);
   r.t_end = r.split.begin(range + 1);
-  int64_t before = 0;
+  int before = 0;
   for (int b0 = b_first; b0 <= b_last; b0 += 32) {
     if (b_last - b_first >= 32) t = tree_lane<SAMPLE>(a, b0, lane, before);     // else it is still in the registers
     const unsigned hit = __ballot_sync(0xffffffffu, t.end > r.t_begin);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int64_t start = __shfl_sync(0xffffffffu, t.end - t.all, src);
-      const int64_t skip = (r.t_begin - start) / __shfl_sync(0xffffffffu, t.tiles, src);
-      r.g = __shfl_sync(0xffffffffu, t.first, src) + (int)skip;
+      const int start = __shfl_sync(0xffffffffu, t.end - t.all, src);
+      const int skip = (r.t_begin - start) / __shfl_sync(0xffffffffu, t.tiles, src);
+      r.g = __shfl_sync(0xffffffffu, t.first, src) + skip;
       r.first = start + skip * __shfl_sync(0xffffffffu, t.tiles, src);
       break;
     }
@@ -159,31 +160,39 @@ __device__ __forceinline__ TreeRange tree_range(const TreeArgs& a, int range, in
 // Warp-cooperative: the launch's split, and the first tile of group g.
 struct TreeGroup {
   TreeSplit split;
-  int64_t first;
+  int first;
 };
 __device__ __forceinline__ TreeGroup tree_group(const TreeArgs& a, int g, int lane) {
   const int H = a.c.kv_heads, b_first = a.g0 / H, b_last = (a.g1 - 1) / H, b = g / H;
   TreeGroup r;
-  int64_t W = 0;
+  int W = 0;
   r.first = 0;
   for (int b0 = b_first; b0 <= b_last; b0 += 32) {
     const TreeLane t = tree_lane<false>(a, b0, lane, W);
     if (b >= b0 && b < b0 + 32)
       r.first = __shfl_sync(0xffffffffu, t.end - t.all, b - b0) +
-                (int64_t)(g - __shfl_sync(0xffffffffu, t.first, b - b0)) * __shfl_sync(0xffffffffu, t.tiles, b - b0);
+                (g - __shfl_sync(0xffffffffu, t.first, b - b0)) * __shfl_sync(0xffffffffu, t.tiles, b - b0);
     W = __shfl_sync(0xffffffffu, t.end, 31);
   }
   r.split.W = W;
-  r.split.N = (int)min((int64_t)a.ranges, W);
+  r.split.N = min(a.ranges, W);
   return r;
 }
 
 // Where list s of a row's part begins in the row's region: the part-th piece of the group, `tiles` tiles from `tile0`.
-__device__ __forceinline__ int64_t tree_list_place(const TreeArgs& a, int64_t tile0, int part, int64_t tiles, int s) {
-  return (tile0 + (int64_t)part * (a.list_turn - 1)) * kTreeTile +
-         s * ((tiles + a.list_turn - 1) / a.list_turn) * a.list_cols;
+__device__ __forceinline__ int tree_list_place(const TreeArgs& a, int tile0, int part, int tiles, int s) {
+  return (tile0 + part * (a.list_turn - 1)) * kTreeTile + s * ((tiles + a.list_turn - 1) / a.list_turn) * a.list_cols;
 }
 
+// Programmatic launches: a kernel may start while the one before it still runs, up to the point where it needs its results.
+__device__ __forceinline__ void tree_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void tree_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {      // a NaN stays
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));

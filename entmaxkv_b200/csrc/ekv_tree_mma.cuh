@@ -32,12 +32,10 @@ constexpr int kTmThreads = (kTmMmaWarp + 1) * 32;
 constexpr int kTmMaxRows = 256;        // rows per block
 constexpr int kTmMaxStages = 6;
 constexpr int kTmMaxAcc = 4;           // accumulators
-constexpr int kTmClasses = 32;         // class maxima per thread
 
 enum TmMode { TM_SAMPLE, TM_LISTS, TM_DENSE };
 
 struct TmSmem {                        // behind the operand tiles
-  float thr[kTmMaxRows];               // raw score units (before zscale)
   uint64_t full[kTmMaxStages], empty[kTmMaxStages], acc_full[kTmMaxAcc], acc_empty[kTmMaxAcc], q_full;
   uint32_t tmem;
   int abort;
@@ -148,80 +146,49 @@ __device__ __forceinline__ float tm_pick(const float (&v)[16], int j) {
 }
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kTmEpiThreads) : "memory"); }
 
-// sum (t_i - mid)_+^beta over the lane's values
-template <int KIND>
-__device__ __forceinline__ float tm_sum(const float (&t)[kTmClasses], float mid, float beta) {
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kTmClasses; ++i) {
-    const float d = fmaxf(t[i] - mid, 0.f);
-    if (KIND == 0) sum += d;
-    else if (KIND == 1) sum = fmaf(d, d, sum);
-    else if (d > 0.f) sum += pow_pos(d, beta);
-  }
-  return sum;
-}
-// A lower bound of the tau of the scores t (z units; -inf: none) that `width` neighbouring lanes hold 32 each, by
-// bisection that keeps its lower end.  Every lane of the warp takes part.
-template <int KIND>
-__device__ __forceinline__ float tm_bound(const float (&t)[kTmClasses], int width, float alpha) {
-  float top = t[0];
-#pragma unroll
-  for (int i = 1; i < kTmClasses; ++i) top = max_nan(top, t[i]);
-  for (int o = width / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float beta = 1.f / (alpha - 1.f);
-  float lo = top - 1.f, hi = top;
-#pragma unroll 1
-  for (int it = 0; it < 6; ++it) {
-    const float mid = 0.5f * (lo + hi);
-    float sum = tm_sum<KIND>(t, mid, beta);
-    for (int o = width / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (sum >= 1.f) lo = mid; else hi = mid;
-  }
-  if (!(fabsf(top) < INFINITY)) return top == INFINITY ? INFINITY : -INFINITY;   // a NaN: everything is a candidate
-  // the roundings of the scaling (2^-24 each) and of the sum: its relative error of 256 2^-24 moves tau by at most
-  // (alpha - 1) 256 2^-24, as sum d^(beta-1) >= 1 where sum d^beta = 1
-  return lo - 2e-5f * alpha * (fabsf(top) + 1.f);
-}
-
-// The rows' bounds from the sample, by all epilogue threads.  (A call: inlined, its 32 class maxima per thread make the
-// pass over K spill registers.)
-static __device__ __noinline__ void tm_sample_bounds(const TreeArgs& a, float* thr, int64_t row_id, int live, int n_rows,
-                                                     int n_classes) {
-  const int tid = threadIdx.x;
-  // 2..32 lanes share a row's class maxima, 32 each; more than that many are folded by maximum
-  int width = 2;
-  while (width < 32 && width * 2 * n_rows <= kTmEpiThreads) width *= 2;
-  const int part_of = tid % width;
-  for (int r0 = 0; r0 < live; r0 += kTmEpiThreads / width) {
-    const int row = r0 + tid / width;
-    const float4* const cls = reinterpret_cast<const float4*>(a.classes + (row_id + min(row, live - 1)) * a.sample_tiles * 4);
-    float t[kTmClasses];
-#pragma unroll
-    for (int i = 0; i < kTmClasses; ++i) t[i] = -INFINITY;
-    for (int f = 0; f < n_classes; f += kTmClasses * width)
-#pragma unroll
-      for (int i = 0; i < kTmClasses; i += 4) {
-        const int q4 = (f + i * width) / 4 + part_of;
-        if (q4 * 4 < n_classes) {
-          const float4 v = cls[q4];
-          t[i] = max_nan(t[i], v.x);
-          t[i + 1] = max_nan(t[i + 1], v.y);
-          t[i + 2] = max_nan(t[i + 2], v.z);
-          t[i + 3] = max_nan(t[i + 3], v.w);
-        }
-      }
-#pragma unroll
-    for (int i = 0; i < kTmClasses; ++i) t[i] *= a.zscale;
-    const int kind = alpha_kind_of(a.alpha);
-    const float bound = kind == 0 ? tm_bound<0>(t, width, a.alpha)
-                                  : (kind == 1 ? tm_bound<1>(t, width, a.alpha) : tm_bound<2>(t, width, a.alpha));
-    if (part_of == 0 && row < live) thr[row] = bound / a.zscale;
-  }
-}
-
 __host__ __device__ inline size_t tm_smem_bytes(int row_tiles, int head_dim, int stages) {
   return 1024 + (size_t)(row_tiles + stages) * kTreeTile * head_dim * 2 + sizeof(TmSmem);
+}
+
+// The rows' bounds from the sample: a warp per row; each lane folds its share of the class maxima into 16, and bisection
+// that keeps its lower end gives a bound of the tau of all of them.
+__global__ void __launch_bounds__(256) tree_bounds_kernel(const __grid_constant__ TreeArgs a, const int64_t n_rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  tree_let_next_start();
+  if (id >= n_rows) return;
+  const int b = (a.g0 + (int)(id / a.rows)) / a.c.kv_heads;
+  const int n = tree_tiles<true>(a, b) * 4;
+  const bool live = (a.row0 + (int)(id % a.rows)) / a.group < tree_drafts(a, b);
+  tree_wait_for_previous();
+  if (!live || n == 0) return;
+  const float* const cls = a.classes + id * a.sample_tiles * 4;
+  float t[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    t[i] = -INFINITY;
+    for (int c = i * 32 + lane; c < n; c += 512) t[i] = max_nan(t[i], cls[c]);
+  }
+  float top = t[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) top = max_nan(top, t[i]);
+  top = warp_max_nan(top) * a.zscale;
+  const int kind = alpha_kind_of(a.alpha);
+  const float beta = 1.f / (a.alpha - 1.f);
+  float lo = top - 1.f, hi = top;
+#pragma unroll 1
+  for (int it = 0; it < 8; ++it) {
+    const float mid = 0.5f * (lo + hi);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += entmax_weight(t[i] * a.zscale, mid, kind, beta);
+    if (warp_sum(sum) >= 1.f) lo = mid; else hi = mid;
+  }
+  // the roundings of the scaling (2^-24 each) and of the sum: its relative error of 512 2^-24 moves tau by at most
+  // (alpha - 1) 512 2^-24, as sum d^(beta-1) >= 1 where sum d^beta = 1.  A NaN: everything is a candidate
+  float bound = (lo - 4e-5f * a.alpha * (fabsf(top) + 1.f)) / a.zscale;
+  if (!(fabsf(top) < INFINITY)) bound = top == INFINITY ? INFINITY : -INFINITY;
+  if (lane == 0) a.row_bounds[id] = bound;
 }
 
 // grid: ranges * row_blocks
@@ -242,9 +209,13 @@ __global__ void __launch_bounds__(kTmThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int range = blockIdx.x / a.row_blocks, rb = blockIdx.x % a.row_blocks;
   const int H = a.c.kv_heads;
+  tree_let_next_start();
   const TreeRange at = tree_range<SAMPLE>(a, range, lane);
-  if (at.t_begin == at.t_end) return;
-  const int64_t t_begin = at.t_begin, t_end = at.t_end;
+  if (at.t_begin == at.t_end) {
+    if (MODE == TM_LISTS) tree_wait_for_previous();        // nothing ends before what it was launched behind
+    return;
+  }
+  const int t_begin = at.t_begin, t_end = at.t_end;
   const int row_first = a.row0 + rb * sh.n_rows;
   const int n_acc = sh.row_tiles == 2 ? 2 : 4, acc_cols = sh.row_tiles * kTreeTile;      // 512 columns: all of TMEM
 
@@ -274,7 +245,7 @@ __global__ void __launch_bounds__(kTmThreads, 1)
   const uint32_t tmem = s->tmem;
 
   // the pieces of groups that this block scores: every role walks them alike
-  int64_t g_first = at.first;
+  int g_first = at.first;
   TmRing stage, acc_ring;
   int n = 0;                                               // tiles so far
   int segment = 0;
@@ -282,7 +253,7 @@ __global__ void __launch_bounds__(kTmThreads, 1)
     const int b = g / H, hkv = g % H;
     const int g_tiles = tree_tiles<SAMPLE>(a, b);
     if (g_tiles == 0) continue;
-    const int tile0 = (int)(max(t_begin, g_first) - g_first), tile1 = (int)(min(t_end, g_first + g_tiles) - g_first);
+    const int tile0 = max(t_begin, g_first) - g_first, tile1 = min(t_end, g_first + g_tiles) - g_first;
     const int part = range - at.split.piece_of(g_first);
     const int len = tree_len(a, b), all_tiles = tree_all_tiles(a, b);
     const int live = min(tree_drafts(a, b) * a.group - row_first, min(a.rows - rb * sh.n_rows, sh.n_rows));
@@ -294,7 +265,7 @@ __global__ void __launch_bounds__(kTmThreads, 1)
       const int quad = warp & 3, wg = warp >> 2;
       const int64_t row_id = (int64_t)(g - a.g0) * a.rows + rb * sh.n_rows;
       const int per_copy = kTreeTile / sh.copies;          // lanes of a copy
-      epi_sync();                                          // the previous segment's bounds have been used
+      epi_sync();
       // the previous segment's products have all run (their accumulators were read): its rows may go
       for (int i = tid; i < sh.row_tiles * kTreeTile * CPR; i += kTmEpiThreads) {
         const int slot = i / CPR, c = i % CPR, in_tile = slot % kTreeTile;
@@ -310,10 +281,7 @@ __global__ void __launch_bounds__(kTmThreads, 1)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // plain stores, read by the tensor core
       epi_sync();
       if (tid == 0) tm_arrive(&s->q_full);
-      if (MODE == TM_LISTS) {
-        tm_sample_bounds(a, s->thr, row_id, live, sh.n_rows, tree_tiles<true>(a, b) * 4);
-        epi_sync();
-      }
+      if (MODE == TM_LISTS && segment == 0) tree_wait_for_previous();    // the bounds; K and the rows need no waiting
       // this thread's row, its columns, and which tiles are its warpgroup's
       const int row_tile = sh.row_tiles == 2 ? wg & 1 : 0;
       const int in_tile = quad * 32 + lane, row = row_tile * kTreeTile + in_tile % per_copy;
@@ -321,7 +289,7 @@ __global__ void __launch_bounds__(kTmThreads, 1)
       const int col0 = sh.row_tiles == 2 ? (wg >> 1) * cols : in_tile / per_copy * cols;
       const int turn = sh.row_tiles == 2 ? 1 : 4;          // a warpgroup takes every turn-th tile
       const bool ok = row < live;
-      const float thr = MODE == TM_LISTS && ok ? s->thr[row] : INFINITY;
+      const float thr = MODE == TM_LISTS && ok ? a.row_bounds[row_id + row] : INFINITY;
       const int list = sh.row_tiles == 2 ? wg >> 1 : in_tile / per_copy * 4 + wg;
       uint2* const out = a.entries + (row_id + (ok ? row : 0)) * a.region;
       uint2* const first = MODE == TM_LISTS ? out + tree_list_place(a, tile0, part, tile1 - tile0, list) : nullptr;
@@ -454,6 +422,7 @@ __global__ void __launch_bounds__(kTmThreads, 1)
       }
     __syncwarp();
   }
+  if (MODE == TM_LISTS) tree_wait_for_previous();
   tm_fence_before();
   __syncthreads();
   tm_fence_after();
