@@ -1,9 +1,11 @@
 // Several tokens per sequence written into the cache, with the statistics of every page that they touch.
 //
 // Row i < counts[b] of sequence b is row index[b, i] (or i) of k_new / v_new and lands at position start[b] + i.  A page
-// is handled by LPR lanes, one 16-byte column each: the lane gathers the page's rows - those already in the cache and
-// the new ones - into registers, stores the new ones, and forms the column's statistics from the same registers, so each
-// new row is read once and written once and an old row is read only where it shares the first page.  Bound by memory.
+// of keys is handled by LPR lanes, one 16-byte column each: a lane gathers the page's rows - those already in the cache
+// and the new ones, 16 on their way at a time - stores the new ones and forms the column's statistics from the same
+// registers, so a new row is read once and written once and an old row is read only where it shares the first page.
+// Values are copied by blocks of their own: with both in one thread the registers leave too few loads in flight.
+// Bound by memory.
 #include "ekv_page_stats.cuh"
 
 namespace ekv {
@@ -21,12 +23,12 @@ struct ExtendArgs {
   int* status;
 };
 
-constexpr int kExtendThreads = 256;
+constexpr int kExtendMaxThreads = 256;
 constexpr int kExtendRows = 16;  // rows of a page held in registers at once
 
-// grid: (B * H_kv, page groups)
+// grid: (B * H_kv, page groups, 2: keys, values)
 template <typename T, int D>
-__global__ void __launch_bounds__(kExtendThreads) extend_kernel(const __grid_constant__ ekv_cache_desc c,
+__global__ void __launch_bounds__(kExtendMaxThreads) extend_kernel(const __grid_constant__ ekv_cache_desc c,
                                                                 const __grid_constant__ ExtendArgs a) {
   constexpr int EPL = ElemTraits<T>::EPL;
   constexpr int LPR = D / EPL;
@@ -50,76 +52,60 @@ __global__ void __launch_bounds__(kExtendThreads) extend_kernel(const __grid_con
   }
   const int end = start + n;
   const int page0 = start / P;
-  const int64_t page64 = page0 + ((int64_t)blockIdx.y * kExtendThreads + threadIdx.x) / LPR;
+  const int64_t page64 = page0 + ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) / LPR;
   const int col = threadIdx.x % LPR * EPL;
   // a rewind without new rows still leaves its page with fewer rows
   if (page64 * P < end && (n > 0 || start < now)) {
     const int page = (int)page64;
     size_t off;
     if (kv_page_offset(c, b, h, page, off)) {
-      T* const kb = static_cast<T*>(c.k) + off + col;
-      T* const vb = static_cast<T*>(c.v) + off + col;
-      const T* const kn = static_cast<const T*>(a.k_new) + b * a.sb + h * a.sh + col;
-      const T* const vn = static_cast<const T*>(a.v_new) + b * a.sb + h * a.sh + col;
+      const bool keys = blockIdx.z == 0;
+      T* const to = static_cast<T*>(keys ? c.k : c.v) + off + col;
+      const T* const from = static_cast<const T*>(keys ? a.k_new : a.v_new) + b * a.sb + h * a.sh + col;
       const int64_t r0 = (int64_t)page * P;
       const int rows = (int)min((int64_t)P, end - r0);
-      auto source = [&](int64_t pos) -> int64_t {      // element offset of the new row at position pos
-        int i = (int)(pos - start);
+      const int old = (int)min(max(start - r0, (int64_t)0), (int64_t)rows);      // rows that are in the cache
+      const auto source = [&](int i) -> const T* {     // the new row that becomes row i of the page
+        int j = (int)(r0 + i - start);
         if (a.index) {
-          const int j = a.index[b * a.index_sb + i];
-          i = min(max(j, 0), a.tokens - 1);
-          if (i != j) flag |= EKV_STATUS_TOKENS;
+          const int given = a.index[b * a.index_sb + j];
+          j = min(max(given, 0), a.tokens - 1);
+          if (j != given) flag |= EKV_STATUS_TOKENS;
         }
-        return i * a.st;
+        return from + j * a.st;
       };
+      uint4 x[kExtendRows];
       ColumnStats<T> st;
       st.begin();
-      if (rows <= kExtendRows) {
-        uint4 k[kExtendRows], v[kExtendRows];
+      for (int i0 = keys ? 0 : old; i0 < rows; i0 += kExtendRows) {
+        const int n = min(rows - i0, kExtendRows);
 #pragma unroll
         for (int i = 0; i < kExtendRows; ++i)
-          if (i < rows) {
-            if (r0 + i < start) {
-              k[i] = *reinterpret_cast<const uint4*>(kb + (size_t)i * D);
-            } else {
-              const int64_t s = source(r0 + i);
-              k[i] = ld_stream(kn + s);
-              v[i] = ld_stream(vn + s);
-            }
-          }
+          if (i < n) x[i] = i0 + i < old ? *reinterpret_cast<const uint4*>(to + (size_t)(i0 + i) * D) : ld_stream(source(i0 + i));
 #pragma unroll
         for (int i = 0; i < kExtendRows; ++i)
-          if (i < rows) {
-            if (r0 + i >= start) {
-              *reinterpret_cast<uint4*>(kb + (size_t)i * D) = k[i];
-              *reinterpret_cast<uint4*>(vb + (size_t)i * D) = v[i];
-            }
-            st.first_pass(k[i]);
+          if (i < n) {
+            if (i0 + i >= old) *reinterpret_cast<uint4*>(to + (size_t)(i0 + i) * D) = x[i];
+            if (keys) st.first_pass(x[i]);
           }
-        st.middle((float)rows);
-#pragma unroll
-        for (int i = 0; i < kExtendRows; ++i)
-          if (i < rows) st.second_pass(k[i]);
-      } else {
-        for (int i = 0; i < rows; ++i) {
-          uint4 k;
-          if (r0 + i < start) {
-            k = *reinterpret_cast<const uint4*>(kb + (size_t)i * D);
-          } else {
-            const int64_t s = source(r0 + i);
-            k = ld_stream(kn + s);
-            *reinterpret_cast<uint4*>(kb + (size_t)i * D) = k;
-            *reinterpret_cast<uint4*>(vb + (size_t)i * D) = ld_stream(vn + s);
-          }
-          st.first_pass(k);
-        }
-        st.middle((float)rows);
-        // this lane re-reads only the column that it wrote itself
-        for (int i = 0; i < rows; ++i) st.second_pass(*reinterpret_cast<const uint4*>(kb + (size_t)i * D));
       }
-      const size_t mo = b * c.meta_stride_b + h * c.meta_stride_h + (size_t)page * D + col;
-      st.finish((float)rows, static_cast<T*>(c.k_min) + mo, static_cast<T*>(c.k_max) + mo,
-                static_cast<T*>(c.k_mean) + mo, static_cast<T*>(c.k_std) + mo);
+      if (keys) {
+        st.middle((float)rows);
+        for (int i0 = 0; i0 < rows; i0 += kExtendRows) {
+          const int n = min(rows - i0, kExtendRows);
+          if (rows > kExtendRows) {                    // longer pages: this lane re-reads the column that it wrote itself
+#pragma unroll
+            for (int i = 0; i < kExtendRows; ++i)
+              if (i < n) x[i] = *reinterpret_cast<const uint4*>(to + (size_t)(i0 + i) * D);
+          }
+#pragma unroll
+          for (int i = 0; i < kExtendRows; ++i)
+            if (i < n) st.second_pass(x[i]);
+        }
+        const size_t mo = b * c.meta_stride_b + h * c.meta_stride_h + (size_t)page * D + col;
+        st.finish((float)rows, static_cast<T*>(c.k_min) + mo, static_cast<T*>(c.k_max) + mo,
+                  static_cast<T*>(c.k_mean) + mo, static_cast<T*>(c.k_std) + mo);
+      }
     }
   }
   if (flag) atomicOr(a.status, flag);
@@ -129,13 +115,13 @@ __global__ void __launch_bounds__(kExtendThreads) extend_kernel(const __grid_con
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    s_last = atomicAdd(&a.counters[b], 1) == c.kv_heads * (int)gridDim.y - 1;
+    s_last = atomicAdd(&a.counters[b], 1) == c.kv_heads * (int)(gridDim.y * gridDim.z) - 1;
     s_end = end;
   }
   __syncthreads();
   if (!s_last) return;
   if (c.block_table) {
-    for (int64_t p = page0 + threadIdx.x; p * P < end; p += kExtendThreads) {
+    for (int64_t p = page0 + threadIdx.x; p * P < end; p += blockDim.x) {
       size_t off;
       if (!kv_page_offset(c, b, 0, (int)p, off)) atomicMin(&s_end, (int)max(p * P, (int64_t)start));
     }
@@ -165,11 +151,12 @@ extern "C" int ekv_extend(const ekv_cache_desc* c, const void* k_new, const void
                      start, counters, status};
   const int64_t pages = (int64_t)(tokens - 1) / c->page_size + 2;    // that `tokens` rows can touch
   const int64_t lanes = c->head_dim * esz / 16;
-  const int64_t groups = (pages * lanes + kExtendThreads - 1) / kExtendThreads;
-  if (groups > 65535 || groups * c->kv_heads > 0x7fffffff || (int64_t)c->batch * c->kv_heads > 0x7fffffff)
+  const int threads = pages * lanes >= kExtendMaxThreads ? kExtendMaxThreads : (int)((pages * lanes + 31) / 32 * 32);
+  const int64_t groups = (pages * lanes + threads - 1) / threads;
+  if (groups > 65535 || 2 * groups * c->kv_heads > 0x7fffffff || (int64_t)c->batch * c->kv_heads > 0x7fffffff)
     return EKV_ERR_ARG;
   EKV_DISPATCH(c->dtype, c->head_dim, {
-    extend_kernel<T, D><<<dim3((unsigned)(c->batch * c->kv_heads), (unsigned)groups), kExtendThreads, 0,
+    extend_kernel<T, D><<<dim3((unsigned)(c->batch * c->kv_heads), (unsigned)groups, 2), threads, 0,
                           as_stream(stream)>>>(*c, a);
   });
   return launch_status();

@@ -8,8 +8,9 @@
 // alone would be off by 0.06 rad.
 //
 // Bound by memory (each element read and written once).  A row of D elements is covered by LPR lanes of 16 bytes; a
-// thread keeps its lane of the row for every head that it visits, so the cosines, sines and weights of its eight (four)
-// elements are loaded once and stay in registers, and the angles of a token are computed once per block.
+// thread keeps its lane of the row for every head and token that it visits, so the weights of its eight (four) elements
+// stay in registers, the cosines and sines are read once per token, and four rows are on their way while one is worked
+// on.  A block takes several tokens, whose angles it computes first.
 #include "ekv_common.cuh"
 
 namespace ekv {
@@ -26,7 +27,9 @@ struct RopeArgs {
   int batch, tokens, half;
   int pos64, weight_f32, interleaved, norm;
   float eps;
-  int tokens_per_block, slots_per_token, rows_per_block;   // see rope_launch
+  int side, turns_in_row;      // tokens side by side in a block, and one after another
+  int slots_per_token;         // rows of a token side by side
+  int rows_per_block;
 };
 
 constexpr int kRopeThreads = 256;
@@ -36,34 +39,48 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int EPL = ElemTraits<T>::EPL;
   constexpr int LPR = D / EPL;
-  extern __shared__ float2 s_turn[];                 // [tokens_per_block][half]: cosine, sine
+  extern __shared__ float2 s_turn[];                 // [side * turns_in_row][half]: cosine, sine
   const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
-  const int tok = slot / a.slots_per_token;          // token of this block
-  const int64_t n_tok = (int64_t)a.batch * a.tokens;
-  const int64_t bt = (int64_t)blockIdx.x * a.tokens_per_block + tok;
-  const bool live = tok < a.tokens_per_block && bt < n_tok;
-  const int b = live ? (int)(bt / a.tokens) : 0, t = live ? (int)(bt % a.tokens) : 0;
+  const int tok = slot / a.slots_per_token, place = slot % a.slots_per_token;
+  const int per_block = a.side * a.turns_in_row;     // tokens of this block
+  const int64_t n_tok = (int64_t)a.batch * a.tokens, bt0 = (int64_t)blockIdx.x * per_block;
   const int all = a.heads[0] + a.heads[1];
   const int first = blockIdx.y * a.rows_per_block, last = min(first + a.rows_per_block, all);
+  const int per_token = (last - first + a.slots_per_token - 1) / a.slots_per_token;     // rows of a thread in a token
   const int e0 = lane * EPL;
 
-  auto row_in = [&](int r) -> const uint4* {
-    const int w = r >= a.heads[0];
-    const int h = r - (w ? a.heads[0] : 0);
-    return reinterpret_cast<const uint4*>(static_cast<const T*>(a.x[w]) + b * a.xs[w][0] + h * a.xs[w][1] +
-                                          t * a.xs[w][2] + e0);
+  // this thread's rows, token after token: a place in that sequence
+  struct At {
+    int turn, i;
+  };
+  const auto step = [&](At& at) {
+    if (++at.i == per_token) {
+      at.i = 0;
+      ++at.turn;
+    }
+  };
+  const auto row_of = [&](const At& at) { return first + place + at.i * a.slots_per_token; };
+  const auto token_of = [&](const At& at) { return bt0 + at.turn * a.side + tok; };
+  const auto live = [&](const At& at) {
+    return at.turn < a.turns_in_row && tok < a.side && row_of(at) < last && token_of(at) < n_tok;
+  };
+  const auto load = [&](const At& at) -> uint4 {
+    if (!live(at)) return make_uint4(0, 0, 0, 0);
+    const unsigned bt = (unsigned)token_of(at), b = bt / (unsigned)a.tokens, t = bt - b * a.tokens;
+    const int r = row_of(at), w = r >= a.heads[0], h = r - (w ? a.heads[0] : 0);
+    return __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x[w]) + b * a.xs[w][0] + h * a.xs[w][1] +
+                                                 t * a.xs[w][2] + e0));
   };
   // the first rows are on their way while the angles are computed
   uint4 raw[kRopeFlight];
-  const int r0 = first + slot % a.slots_per_token;
+  At ahead{0, 0};
 #pragma unroll
   for (int i = 0; i < kRopeFlight; ++i) {
-    const int r = r0 + i * a.slots_per_token;
-    raw[i] = live && r < last ? __ldcs(row_in(r)) : make_uint4(0, 0, 0, 0);
+    raw[i] = load(ahead);
+    step(ahead);
   }
-
-  for (int i = threadIdx.x; i < a.tokens_per_block * a.half; i += kRopeThreads) {
-    const int64_t at = (int64_t)blockIdx.x * a.tokens_per_block + i / a.half;
+  for (int i = threadIdx.x; i < per_block * a.half; i += kRopeThreads) {
+    const int64_t at = bt0 + i / a.half;
     if (at < n_tok) {
       const int64_t off = at / a.tokens * a.ps_b + at % a.tokens * a.ps_t;
       const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[off]
@@ -72,23 +89,6 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
       float2 cs;
       sincospif(2.f * (float)(turns - rint(turns)), &cs.y, &cs.x);
       s_turn[i] = cs;
-    }
-  }
-  __syncthreads();
-
-  const bool turned = e0 < 2 * a.half;                       // a lane is rotated as a whole or not at all
-  const bool upper = !a.interleaved && e0 >= a.half;
-  float co[EPL], si[EPL];
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    co[j] = 1.f;
-    si[j] = 0.f;
-    if (turned && live) {
-      const int p = a.interleaved ? (e0 + j) / 2 : (upper ? e0 + j - a.half : e0 + j);
-      const float2 cs = s_turn[tok * a.half + p];
-      co[j] = cs.x;
-      // y_a' = y_a cos - y_b sin;  y_b' = y_b cos + y_a sin
-      si[j] = a.interleaved ? (j & 1 ? cs.y : -cs.y) : (upper ? cs.y : -cs.y);
     }
   }
   float w[2][EPL];
@@ -101,28 +101,46 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
                                      : to_float<T>(static_cast<const T*>(a.weight[which])[e0 + j]);
     }
   }
+  const bool turned = e0 < 2 * a.half;                       // a lane is rotated as a whole or not at all
+  const bool upper = !a.interleaved && e0 >= a.half;
+  const int pair0 = a.interleaved ? e0 / 2 : (upper ? e0 - a.half : e0);
   const int warp_lane = threadIdx.x & 31;
   const int partner = a.interleaved || !turned ? warp_lane
                       : upper                  ? warp_lane - a.half / EPL
                                                : warp_lane + a.half / EPL;
+  __syncthreads();
 
-  for (int base = first; base < last; base += kRopeFlight * a.slots_per_token) {
+  float co[EPL], si[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    co[j] = 1.f;
+    si[j] = 0.f;
+  }
+  At at{0, 0};
+  for (int done = 0; done < a.turns_in_row * per_token; done += kRopeFlight) {
 #pragma unroll
     for (int i = 0; i < kRopeFlight; ++i) {
-      if (base + i * a.slots_per_token >= last) break;       // uniform over the block
-      const int r = base + slot % a.slots_per_token + i * a.slots_per_token;
-      const int which = r >= a.heads[0];
-      float x[EPL];
+      if (done + i >= a.turns_in_row * per_token) break;     // uniform over the block
+      if (at.i == 0 && turned && tok < a.side) {             // a new token: y_a' = y_a cos - y_b sin; y_b' = y_b cos + y_a sin
+        const float2* const cs = s_turn + (at.turn * a.side + tok) * a.half + pair0;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+          const float2 c = cs[a.interleaved ? j / 2 : j];
+          co[j] = c.x;
+          si[j] = a.interleaved ? (j & 1 ? c.y : -c.y) : (upper ? c.y : -c.y);
+        }
+      }
+      const bool ok = live(at);
+      const int r = row_of(at), which = r >= a.heads[0];
+      float x[EPL], other[EPL];
       unpack<T>(raw[i], x);
       float scale = 1.f;
       if (a.norm) {
         float sq = 0.f;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) sq = fmaf(x[j], x[j], sq);
-        sq = row_sum<LPR>(sq);
-        scale = 1.f / sqrtf(sq * (1.f / D) + a.eps);
+        scale = rsqrtf(row_sum<LPR>(sq) * (1.f / D) + a.eps);
       }
-      float other[EPL];
 #pragma unroll
       for (int j = 0; j < EPL; ++j) x[j] = x[j] * scale * (which ? w[1][j] : w[0][j]);
       if (a.interleaved) {
@@ -132,19 +150,19 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
 #pragma unroll
         for (int j = 0; j < EPL; ++j) other[j] = __shfl_sync(0xffffffffu, x[j], partner);
       }
-      if (!turned) {                                         // an infinity outside the rotated part stays what it is
+      if (turned) {                                          // an infinity outside the rotated part stays what it is
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) other[j] = 0.f;
+        for (int j = 0; j < EPL; ++j) x[j] = fmaf(x[j], co[j], other[j] * si[j]);
       }
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) x[j] = fmaf(x[j], co[j], other[j] * si[j]);
-      if (live && r < last) {
+      if (ok) {
+        const unsigned bt = (unsigned)token_of(at), b = bt / (unsigned)a.tokens, t = bt - b * a.tokens;
         const int h = r - (which ? a.heads[0] : 0);
         *reinterpret_cast<uint4*>(static_cast<T*>(a.y[which]) + b * a.ys[which][0] + h * a.ys[which][1] +
                                   t * a.ys[which][2] + e0) = pack<T>(x);
       }
-      const int next = r + kRopeFlight * a.slots_per_token;
-      if (live && next < last) raw[i] = __ldcs(row_in(next));
+      raw[i] = load(ahead);
+      step(ahead);
+      step(at);
     }
   }
 }
@@ -200,15 +218,25 @@ extern "C" int ekv_qk_norm_rope(int32_t dtype, int32_t batch, int32_t tokens, in
   const int slots = kRopeThreads / (int)(head_dim * esz / 16);       // rows that a block handles side by side
   const int all = q_heads + kv_heads;
   const int64_t n_tok = (int64_t)batch * tokens;
-  // few heads: several tokens share a block.  Many: one token's rows take several turns.
-  a.tokens_per_block = all >= slots ? 1 : slots / all;
-  a.slots_per_token = slots / a.tokens_per_block;
-  // few tokens: the rows of a token are spread over blocks, one turn each (a decode step is latency)
-  const int64_t blocks = (n_tok + a.tokens_per_block - 1) / a.tokens_per_block;
-  a.rows_per_block = blocks >= 2 * sm_count() ? all : a.slots_per_token;
-  const int parts = (all + a.rows_per_block - 1) / a.rows_per_block;
+  if (n_tok > 0x7fffffff) return EKV_ERR_ARG;
+  // few heads: several tokens side by side.  Many: one token's rows take several turns.
+  a.side = all >= slots ? 1 : slots / all;
+  a.slots_per_token = slots / a.side;
+  const int64_t want = 8 * sm_count();               // blocks that fill the GPU
+  const int64_t sides = (n_tok + a.side - 1) / a.side;
+  // few tokens: the rows of a token are spread over blocks (a decode step is latency); many: a block takes several
+  // tokens, whose angles it then computes side by side
+  const int64_t turns = (all + a.slots_per_token - 1) / a.slots_per_token;
+  int64_t parts = want / sides > 1 ? want / sides : 1;
+  if (parts > turns) parts = turns;
+  a.rows_per_block = (int)((turns + parts - 1) / parts) * a.slots_per_token;
+  parts = (all + a.rows_per_block - 1) / a.rows_per_block;
+  int64_t in_row = sides / (2 * want);
+  in_row = in_row < 1 ? 1 : (in_row > 8 ? 8 : in_row);
+  a.turns_in_row = (int)in_row;
+  const int64_t blocks = (sides + in_row - 1) / in_row;
   if (blocks > 0x7fffffff || parts > 65535) return EKV_ERR_ARG;
-  const size_t smem = sizeof(float2) * (size_t)a.tokens_per_block * half;
+  const size_t smem = sizeof(float2) * (size_t)(a.side * in_row) * half;
   EKV_DISPATCH(dtype, head_dim, {
     qk_norm_rope_kernel<T, D><<<dim3((unsigned)blocks, (unsigned)parts), kRopeThreads, smem, as_stream(stream)>>>(a);
   });

@@ -108,11 +108,13 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
 
 // ---- tau and output ------------------------------------------------------------------------------------------------
 //
-// A warp per row while at most 1024 candidates lie above the row's best bound (the usual case: no barrier, sums by
-// shuffle), the whole block per row where more do (flat scores), one such row after another.
+// A warp per row while at most 768 candidates lie above the row's best bound (the usual case: no barrier, sums by
+// shuffle), the whole block per row where more do (flat scores), one such row after another.  Few rows (fewer warps than
+// the GPU holds blocks) get a block each from the start.
 
-constexpr int kFinThreads = 256, kFinWarps = kFinThreads / 32;
-constexpr int kFinLight = 1024;                 // survivors of a row that one warp finishes
+constexpr int kFinWarps = 4;                    // warps of a block that takes a row per warp
+constexpr int kFinOneWarps = 8;                 // and of one that takes a single row
+constexpr int kFinLight = 768;                  // survivors of a row that one warp finishes
 constexpr int kFinLists = 256;                  // and its lists
 constexpr int kFinSlots = kFinWarps * kFinLight;   // of a heavy row on chip; more stay in the row's region
 
@@ -128,7 +130,7 @@ struct FinRow {
 __device__ __forceinline__ FinRow fin_row(const TreeArgs& a, int64_t id, int lane) {
   FinRow r;
   r.id = id;
-  const int g = a.g0 + (int)(id / a.rows), row = a.row0 + (int)(id % a.rows);
+  const int gl = (int)((unsigned)id / (unsigned)a.rows), row = a.row0 + (int)id - gl * a.rows, g = a.g0 + gl;
   r.b = g / a.c.kv_heads;
   r.hkv = g % a.c.kv_heads;
   r.hq = r.hkv * a.group + row % a.group;
@@ -153,50 +155,109 @@ __device__ __forceinline__ int2 fin_list(const TreeArgs& a, const FinRow& r, int
   const int t1 = min(r.split.begin(r.piece0 + p + 1), r.first + r.tiles) - r.first;
   return make_int2(before + count, tree_list_place(a, t0, p, t1 - t0, s) - before);
 }
-// entry i of the concatenation of the row's lists (or of all its scores)
-__device__ __forceinline__ uint2 fin_entry(const TreeArgs& a, const FinRow& r, const int2* lists, int i) {
-  if (a.dense) return make_uint2(__float_as_uint(reinterpret_cast<const float*>(r.region)[a.region + i]), (uint32_t)i);
+// where entry i of the concatenation of the row's lists lies in its region
+__device__ __forceinline__ int fin_place(const FinRow& r, const int2* lists, int i) {
   int lo = 0, hi = r.lists - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (lists[mid].x > i) hi = mid; else lo = mid + 1;
   }
-  return r.region[lists[lo].y + i];
+  return lists[lo].y + i;
 }
-// 16 bytes of the value row of a key (or, ~j, of a drafted token)
-template <typename T, int D>
-__device__ __forceinline__ uint4 fin_value(const TreeArgs& a, const FinRow& r, int key, int col) {
-  const T* v;
-  if (key < 0) {
-    v = static_cast<const T*>(a.v_draft) + r.b * a.vs[0] + r.hkv * a.vs[1] + (int64_t)~key * a.vs[2];
+// N entries of the row, i0 + k * step (those from `raw` on: -inf).  The loads come one after another, without a branch
+// between them: taken one by one their latencies would add up.
+template <int N>
+__device__ __forceinline__ void fin_entries(const TreeArgs& a, const FinRow& r, const int2* lists, int raw, int i0, int step,
+                                            uint2 (&e)[N]) {
+  if (a.dense) {
+    const float* const z = reinterpret_cast<const float*>(r.region) + a.region;
+#pragma unroll
+    for (int k = 0; k < N; ++k) e[k] = make_uint2(__float_as_uint(z[min(i0 + k * step, raw - 1)]), (uint32_t)(i0 + k * step));
   } else {
-    int page, in_page;
-    size_t off;
-    a.by_page.divmod(key, page, in_page);
-    if (!kv_page_offset(a.c, r.b, r.hkv, page, off)) return make_uint4(0, 0, 0, 0);
-    v = static_cast<const T*>(a.c.v) + off + (size_t)in_page * D;
+    int at[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) at[k] = fin_place(r, lists, min(i0 + k * step, raw - 1));
+#pragma unroll
+    for (int k = 0; k < N; ++k) e[k] = r.region[at[k]];
   }
-  return *reinterpret_cast<const uint4*>(v + col);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (i0 + k * step >= raw) e[k].x = __float_as_uint(-INFINITY);
 }
-// Scores of the drafted keys that the row sees (-inf: not), `groups` sets of LPR lanes side by side, this one `mine`.
+// A key's number in the pool (block * page size + place in the page), or itself in a dense cache; -1: no block.  A
+// drafted one (~j) becomes INT_MIN + j.
+__device__ __forceinline__ int fin_pool_key(const TreeArgs& a, const FinRow& r, int key) {
+  if (key < 0) return (int)0x80000000 + ~key;
+  if (!a.c.block_table) return key;
+  int page, in_page;
+  a.by_page.divmod(key, page, in_page);
+  const int block = a.c.block_table[(int64_t)r.b * a.c.bt_stride + page];
+  return (unsigned)block < (unsigned)a.c.num_blocks ? block * a.c.page_size + in_page : -1;
+}
+// 16 bytes of the value rows of N such keys, without a branch between the loads
+template <typename T, int D, int N>
+__device__ __forceinline__ void fin_values(const TreeArgs& a, const FinRow& r, const int (&key)[N], int col, uint4 (&v)[N]) {
+  const T* row[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int at = max(key[k], 0);
+    int64_t off = r.hkv * a.c.kv_stride_h;
+    if (a.c.block_table) {
+      int block, in_page;
+      a.by_page.divmod(at, block, in_page);
+      off += block * a.c.kv_stride_block + (int64_t)in_page * D;
+    } else {
+      off += r.b * a.c.kv_stride_b + (int64_t)at * D;
+    }
+    row[k] = static_cast<const T*>(a.c.v) + off;
+    if (key[k] < -1)
+      row[k] = static_cast<const T*>(a.v_draft) + r.b * a.vs[0] + r.hkv * a.vs[1] + (int64_t)(key[k] & 0x7fffffff) * a.vs[2];
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = *reinterpret_cast<const uint4*>(row[k] + col);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (key[k] == -1) v[k] = make_uint4(0, 0, 0, 0);
+}
+// Scores of the drafted keys that the row sees, the others' are -inf; a warp's share: sets of 32 from `first`, every `step`.
 template <typename T, int D>
-__device__ __forceinline__ void fin_drafts(const TreeArgs& a, const FinRow& r, float* zd, int mine, int groups, int lane) {
-  constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL;
-  const int col = lane % LPR * EPL;
+__device__ __forceinline__ void fin_drafts(const TreeArgs& a, const FinRow& r, float* zd, int lane, int first, int step) {
+  constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL, SIDE = 32 / LPR, N = 4;
+  const int col = lane % LPR * EPL, side = lane / LPR;
   float q[EPL];
   unpack<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + r.b * a.qs[0] + r.hq * a.qs[1] + r.t * a.qs[2] + col), q);
-  const unsigned char* const seen = a.mask + r.b * a.ms_b + r.t * a.ms_t;
+  const unsigned char* const mask = a.mask + r.b * a.ms_b + r.t * a.ms_t;
   const T* const k0 = static_cast<const T*>(a.k_draft) + r.b * a.ks[0] + r.hkv * a.ks[1] + col;
-#pragma unroll 4
-  for (int j0 = 0; j0 < a.tokens; j0 += groups) {
-    const int j = j0 + mine;
-    const bool sees = j < r.drafts && seen[j];
-    float k[EPL], s = 0.f;
-    unpack<T>(sees ? *reinterpret_cast<const uint4*>(k0 + j * a.ks[2]) : make_uint4(0, 0, 0, 0), k);
+  for (int j0 = first * 32; j0 < a.tokens; j0 += step * 32) {
+    const bool sees = j0 + lane < r.drafts && mask[j0 + lane];
+    if (j0 + lane < a.tokens) zd[j0 + lane] = -INFINITY;
+    unsigned left = __ballot_sync(0xffffffffu, sees);
+    __syncwarp();
+    while (left) {                               // SIDE * N of them at a time
+      int j[N];
+      uint4 k[N];
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) s = fmaf(q[e], k[e], s);
-    s = row_sum<LPR>(s);
-    if (lane % LPR == 0 && j < a.tokens) zd[j] = sees ? s * a.zscale : -INFINITY;
+      for (int n = 0; n < N; ++n) {
+        j[n] = -1;
+#pragma unroll
+        for (int s = 0; s < SIDE; ++s) {
+          const int next = __ffs(left) - 1;      // -1: none left
+          if (s == side) j[n] = next;
+          left &= left - 1;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) k[n] = *reinterpret_cast<const uint4*>(k0 + (j0 + max(j[n], 0)) * a.ks[2]);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        float x[EPL], s = 0.f;
+        unpack<T>(k[n], x);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) s = fmaf(q[e], x[e], s);
+        s = row_sum<LPR>(s);
+        if (lane % LPR == 0 && j[n] >= 0) zd[j0 + j[n]] = s * a.zscale;
+      }
+    }
   }
 }
 
@@ -210,8 +271,9 @@ __device__ __forceinline__ float fin_tau(float floor_z, float top, float alpha, 
     const float2 s = sums(tau);
     if (s.x >= 1.f) lo = tau; else hi = tau;
     // (N - 1) / -N' = (s0^(1/beta) - 1) s0^(1 - 1/beta) / s1
-    const float root = kind == 0 ? s.x : (kind == 1 ? sqrtf(s.x) : pow_pos(s.x, alpha - 1.f));
-    const float step = s.x > 0.f ? (root - 1.f) * (s.x / root) / s.y : -INFINITY;
+    // (the step need not be exact: the sums at the new tau decide)
+    const float root = kind == 0 ? s.x : (kind == 1 ? s.x * rsqrtf(s.x) : pow_pos(s.x, alpha - 1.f));
+    const float step = s.x > 0.f ? __fdividef((root - 1.f) * __fdividef(s.x, root), s.y) : -INFINITY;
     // half a unit in the last place of the scores that tau is compared with
     const bool done = fabsf(step) <= 6e-8f * fmaxf(fabsf(tau), fabsf(top));
     const float next = tau + step;
@@ -221,6 +283,7 @@ __device__ __forceinline__ float fin_tau(float floor_z, float top, float alpha, 
   return tau;
 }
 
+template <int WARPS>
 __device__ __forceinline__ float2 block_sum2(float2 v, float* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v.x = warp_sum(v.x);
@@ -233,7 +296,7 @@ __device__ __forceinline__ float2 block_sum2(float2 v, float* scratch) {
   __syncthreads();
   float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < kFinWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     t.x += scratch[w * 2];
     t.y += scratch[w * 2 + 1];
   }
@@ -241,6 +304,7 @@ __device__ __forceinline__ float2 block_sum2(float2 v, float* scratch) {
 }
 
 // exclusive scan of small counts over the block; also the total
+template <int WARPS>
 __device__ __forceinline__ int block_excl(int v, int* scratch, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int inc = v;
@@ -254,7 +318,7 @@ __device__ __forceinline__ int block_excl(int v, int* scratch, int* total) {
   __syncthreads();
   int base = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kFinWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     if (w < warp) base += scratch[w];
     all += scratch[w];
   }
@@ -272,37 +336,195 @@ struct FinHeavy {
 };
 
 // lists in shared memory: kFinLists per warp, or all of one row
-static inline int fin_ends(int max_lists) {
+static inline int fin_lists(int max_lists) {
   const int each = max_lists < kFinLists ? max_lists : kFinLists;
   return each * kFinWarps > max_lists ? each * kFinWarps : max_lists;
 }
 
-// dynamic shared memory: [n_ends] lists, [warps][tokens] drafted scores
+// One row by the whole block.  `lists`: room for all of its lists; `zd`: its drafts' scores, which the caller made.
+template <typename T, int D, int WARPS>
+__device__ void fin_block_row(const TreeArgs& a, const FinRow& r, uint2* s_slots, int2* lists, const float* zd,
+                              float* scratch) {
+  constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL, THREADS = WARPS * 32, GROUPS = THREADS / LPR, N = 4;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kind = alpha_kind_of(a.alpha);
+  const float beta = 1.f / (a.alpha - 1.f);
+  int* const iscratch = reinterpret_cast<int*>(scratch);
+  const FinHeavy rows{s_slots, r.region};
+  const auto block_top = [&](float v) {
+    v = warp_max_nan(v);
+    __syncthreads();
+    if (lane == 0) scratch[warp] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) v = max_nan(v, scratch[w]);
+    return v;
+  };
+  int raw = 0, n = 0;
+  float floor_z = -INFINITY, top = -INFINITY;    // no weight at or below the floor; fmaxf passes over a NaN
+  if (a.dense) {                                 // nothing bounds tau yet: the maximum first
+    raw = r.len;
+    const float* const z = reinterpret_cast<const float*>(r.region) + a.region;
+#pragma unroll 8
+    for (int i = tid; i < raw; i += THREADS) top = max_nan(top, z[i]);
+    for (int j = tid; j < a.tokens; j += THREADS) top = max_nan(top, zd[j]);
+    floor_z = block_top(top) - 1.f;
+    top = -INFINITY;
+  } else {
+    const int* const counts = a.counts + r.id * a.max_parts * a.sub;
+    const float* const bounds = a.bounds + r.id * a.max_parts * a.sub;
+    for (int i0 = 0; i0 < r.lists; i0 += THREADS) {
+      const bool in = i0 + tid < r.lists;
+      const int c = in ? counts[i0 + tid] : 0;
+      if (in) floor_z = fmaxf(floor_z, bounds[i0 + tid]);
+      int total;
+      const int before = block_excl<WARPS>(c, iscratch, &total);
+      if (in) lists[i0 + tid] = fin_list(a, r, i0 + tid, raw + before, c);
+      raw += total;
+    }
+    floor_z = block_max(floor_z, scratch);
+  }
+  __syncthreads();
+  // what lies above the floor, in order; a NaN stays
+  for (int i0 = 0; i0 < raw + a.tokens; i0 += THREADS * N) {
+    uint2 e[N];
+    const int i = i0 + tid * N;
+    if (i0 < raw) {
+      fin_entries(a, r, lists, raw, i, 1, e);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) e[k] = make_uint2(__float_as_uint(-INFINITY), 0);
+    }
+    int mine = 0;
+    bool keep[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = i + k - raw;
+      if (j >= 0 && j < a.tokens) e[k] = make_uint2(__float_as_uint(zd[j]), (uint32_t)~j);     // ~j: drafted
+      const float z = __uint_as_float(e[k].x);
+      keep[k] = !(z <= floor_z);
+      if (keep[k]) top = max_nan(top, z);
+      mine += keep[k];
+    }
+    int total;
+    int at = n + block_excl<WARPS>(mine, iscratch, &total);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (keep[k]) rows.put(at++, e[k]);
+    n += total;
+    __syncthreads();                             // before the next entries are read where these may have been written
+  }
+  top = block_top(top);
+  T* const out = static_cast<T*>(a.out) + r.b * a.os[0] + r.hq * a.os[1] + r.t * a.os[2];
+  float* const tau_out = a.tau ? a.tau + ((int64_t)r.b * a.q_heads + r.hq) * a.tokens + r.t : nullptr;
+  if (!(fabsf(top) < INFINITY)) {                // nothing visible: zeros.  NaN or +inf among the scores: NaN
+    if (tid < D) out[tid] = from_float<T>(top == -INFINITY ? 0.f : NAN);
+    if (tid == 0 && tau_out) *tau_out = top == -INFINITY ? INFINITY : NAN;
+    return;
+  }
+  const float tau = fin_tau(fmaxf(floor_z, top - 1.f), top, a.alpha, kind, [&](float t) {
+    float2 s = make_float2(0.f, 0.f);
+    float s2 = 0.f;
+    for (int i = tid; i < n; i += THREADS) halley_accumulate(__uint_as_float(rows.get(i).x), t, kind, beta, s.x, s.y, s2);
+    return block_sum2<WARPS>(s, scratch);
+  });
+  int m = 0;
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
+    uint2 e = make_uint2(0, 0);
+    float w = 0.f;
+    if (i0 + tid < n) {
+      e = rows.get(i0 + tid);
+      w = entmax_weight(__uint_as_float(e.x), tau, kind, beta);
+    }
+    int total;
+    const int at = m + block_excl<WARPS>(w > 0.f, iscratch, &total);
+    if (w > 0.f) rows.put(at, make_uint2(__float_as_uint(w), (uint32_t)fin_pool_key(a, r, (int)e.y)));
+    m += total;
+  }
+  __syncthreads();
+  float acc[EPL] = {};
+  const int sub = tid / LPR, col = tid % LPR * EPL;
+  for (int i0 = sub; i0 < m; i0 += GROUPS * N) {
+    uint4 v[N];
+    float w[N];
+    int key[N];
+#pragma unroll
+    for (int f = 0; f < N; ++f) {
+      const uint2 e = rows.get(min(i0 + f * GROUPS, m - 1));
+      w[f] = __uint_as_float(e.x);
+      key[f] = (int)e.y;
+    }
+    fin_values<T, D>(a, r, key, col, v);
+#pragma unroll
+    for (int f = 0; f < N; ++f)
+      if (i0 + f * GROUPS < m) {
+        float x[EPL];
+        unpack<T>(v[f], x);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] = fmaf(w[f], x[j], acc[j]);
+      }
+  }
+  __syncthreads();                               // the slots become partial sums
+  float* const s_acc = reinterpret_cast<float*>(s_slots);
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) s_acc[sub * D + col + j] = acc[j];
+  __syncthreads();
+  if (tid < D) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) s += s_acc[i * D + tid];
+    out[tid] = from_float<T>(s);
+  }
+  if (tid == 0 && tau_out) *tau_out = tau;
+}
+
+// A block per row.  Dynamic shared memory: [kFinSlots] slots, [n_lists] lists, [tokens] drafted scores.
 template <typename T, int D>
-__global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __grid_constant__ TreeArgs a, const int64_t n_rows,
-                                                                     const int n_ends) {
-  constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL, SIDE = 32 / LPR, GROUPS = kFinThreads / LPR;
+__global__ void __launch_bounds__(kFinOneWarps * 32) tree_finish_one_kernel(const __grid_constant__ TreeArgs a,
+                                                                            const int n_lists) {
+  extern __shared__ uint2 s_slots[];
+  __shared__ float scratch[32];
+  int2* const lists = reinterpret_cast<int2*>(s_slots + kFinSlots);
+  float* const zd = reinterpret_cast<float*>(lists + n_lists);
+  const int lane = threadIdx.x & 31;
+  const FinRow r = fin_row(a, blockIdx.x, lane);
+  if (r.t < r.drafts) fin_drafts<T, D>(a, r, zd, lane, threadIdx.x >> 5, kFinOneWarps);
+  tree_wait_for_previous();
+  if (r.t >= r.drafts) return;                   // behind a short tree: left as it was
+  __syncthreads();
+  fin_block_row<T, D, kFinOneWarps>(a, r, s_slots, lists, zd, scratch);
+}
+
+// A warp per row.  Dynamic shared memory: [kFinSlots] slots, [n_lists] lists, [warps][tokens] drafted scores.
+template <typename T, int D>
+__global__ void __launch_bounds__(kFinWarps * 32, 7) tree_finish_kernel(const __grid_constant__ TreeArgs a,
+                                                                        const int64_t n_rows, const int n_lists) {
+  constexpr int EPL = ElemTraits<T>::EPL, LPR = D / EPL, SIDE = 32 / LPR;
+  extern __shared__ uint2 s_slots[];
   __shared__ float scratch[32];
   __shared__ int s_heavy[kFinWarps];
-  extern __shared__ uint2 s_slots[];                   // [kFinSlots], then the lists
-  int2* const s_dyn = reinterpret_cast<int2*>(s_slots + kFinSlots);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int2* const lists = s_dyn + warp * min(a.max_parts * a.sub, kFinLists);
-  float* const zd = reinterpret_cast<float*>(s_dyn + n_ends) + warp * a.tokens;
+  int2* const s_lists = reinterpret_cast<int2*>(s_slots + kFinSlots);
+  int2* const lists = s_lists + warp * min(a.max_parts * a.sub, kFinLists);
+  float* const zd = reinterpret_cast<float*>(s_lists + n_lists) + warp * a.tokens;
+  uint2* const slots = s_slots + warp * kFinLight;
   const int64_t id0 = (int64_t)blockIdx.x * kFinWarps;
   const int kind = alpha_kind_of(a.alpha);
   const float beta = 1.f / (a.alpha - 1.f);
 
-  tree_wait_for_previous();
+  // what needs nothing of the score pass
   FinRow r{};
   bool mine = id0 + warp < n_rows, heavy = false;
   if (mine) {
     r = fin_row(a, id0 + warp, lane);
     mine = r.t < r.drafts;                       // else behind a short tree: left as it was
   }
+  if (mine) fin_drafts<T, D>(a, r, zd, lane, 0, 1);
+  tree_wait_for_previous();
+  __syncwarp();
+
   float floor_z = -INFINITY, top = -INFINITY;    // no weight at or below the floor; fmaxf passes over a NaN
   int raw = r.len, n = 0;
-  uint2* const slots = s_slots + warp * kFinLight;
   if (mine) {
     if (!a.dense && r.lists > kFinLists) {
       n = kFinLight + 1;                         // the block's
@@ -325,7 +547,6 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
       }
       floor_z = warp_max(floor_z);
     }
-    fin_drafts<T, D>(a, r, zd, lane / LPR, SIDE, lane);
     __syncwarp();
     // what lies above the floor, in order; a NaN stays.  The floor follows the maximum, and where too much was kept under
     // an early one, the slots are gone through again
@@ -333,12 +554,16 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
     for (int i0 = 0; i0 < raw + a.tokens && n <= kFinLight; i0 += 32 * AT_ONCE) {
       uint2 e[AT_ONCE];
       float most = -INFINITY;
+      if (i0 < raw) {
+        fin_entries(a, r, lists, raw, i0 + lane, 32, e);
+      } else {
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) e[k] = make_uint2(__float_as_uint(-INFINITY), 0);
+      }
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
-        const int i = i0 + 32 * k + lane;
-        e[k] = make_uint2(__float_as_uint(-INFINITY), 0);
-        if (i < raw) e[k] = fin_entry(a, r, lists, i);
-        else if (i < raw + a.tokens) e[k] = make_uint2(__float_as_uint(zd[i - raw]), (uint32_t)~(i - raw));   // ~j: drafted
+        const int j = i0 + 32 * k + lane - raw;
+        if (j >= 0 && j < a.tokens) e[k] = make_uint2(__float_as_uint(zd[j]), (uint32_t)~j);     // ~j: drafted
         most = max_nan(most, __uint_as_float(e[k].x));
       }
       top = max_nan(top, warp_max_nan(most));
@@ -368,26 +593,28 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
     __syncwarp();
   }
   if (lane == 0) s_heavy[warp] = heavy;
-  const auto write = [&](int e, float x) {
-    static_cast<T*>(a.out)[r.b * a.os[0] + r.hq * a.os[1] + r.t * a.os[2] + e] = from_float<T>(x);
-  };
-  const auto write_tau = [&](float x) {
-    if (a.tau) a.tau[((int64_t)r.b * a.q_heads + r.hq) * a.tokens + r.t] = x;
-  };
 
   if (mine && !heavy) {
-    // ---- a warp per row
+    T* const out = static_cast<T*>(a.out) + r.b * a.os[0] + r.hq * a.os[1] + r.t * a.os[2];
+    float* const tau_out = a.tau ? a.tau + ((int64_t)r.b * a.q_heads + r.hq) * a.tokens + r.t : nullptr;
     if (!(fabsf(top) < INFINITY)) {              // nothing visible: zeros.  NaN or +inf among the scores: NaN
-      const float fill = top == -INFINITY ? 0.f : NAN;
-      for (int e = lane; e < D; e += 32) write(e, fill);
-      if (lane == 0) write_tau(top == -INFINITY ? INFINITY : NAN);
+      for (int e = lane; e < D; e += 32) out[e] = from_float<T>(top == -INFINITY ? 0.f : NAN);
+      if (lane == 0 && tau_out) *tau_out = top == -INFINITY ? INFINITY : NAN;
     } else {
-      const float tau = fin_tau(fmaxf(floor_z, top - 1.f), top, a.alpha, kind, [&](float t) {
+      const float tau = fin_tau(floor_z, top, a.alpha, kind, [&](float t) {
         float2 s = make_float2(0.f, 0.f);
         float s2 = 0.f;
+        if (kind == 1) {                         // alpha 1.5, the usual one, without a branch per score
 #pragma unroll 4
-        for (int i = lane; i < n; i += 32)
-          halley_accumulate(__uint_as_float(slots[i].x), t, kind, beta, s.x, s.y, s2);
+          for (int i = lane; i < n; i += 32) {
+            const float d = fmaxf(__uint_as_float(slots[i].x) - t, 0.f);
+            s.x = fmaf(d, d, s.x);
+            s.y += d;
+          }
+        } else {
+          for (int i = lane; i < n; i += 32)
+            halley_accumulate(__uint_as_float(slots[i].x), t, kind, beta, s.x, s.y, s2);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
           s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
@@ -409,23 +636,26 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
         m += __popc(has);
         __syncwarp();
       }
+      if (a.c.block_table)                       // 32 table entries at a time instead of one before each value row
+        for (int i = lane; i < m; i += 32) slots[i].y = (uint32_t)fin_pool_key(a, r, (int)slots[i].y);
+      else
+        for (int i = lane; i < m; i += 32)
+          if ((int)slots[i].y < 0) slots[i].y = (uint32_t)fin_pool_key(a, r, (int)slots[i].y);
+      __syncwarp();
       float acc[EPL] = {};
       const int col = lane % LPR * EPL;
       constexpr int FLIGHT = 4;
       for (int i0 = lane / LPR; i0 < m; i0 += SIDE * FLIGHT) {
         uint4 v[FLIGHT];
         float w[FLIGHT];
+        int key[FLIGHT];
 #pragma unroll
         for (int f = 0; f < FLIGHT; ++f) {
-          const int i = i0 + f * SIDE;
-          w[f] = 0.f;
-          v[f] = make_uint4(0, 0, 0, 0);
-          if (i < m) {
-            const uint2 e = slots[i];
-            w[f] = __uint_as_float(e.x);
-            v[f] = fin_value<T, D>(a, r, (int)e.y, col);
-          }
+          const uint2 e = slots[min(i0 + f * SIDE, m - 1)];
+          w[f] = __uint_as_float(e.x);
+          key[f] = (int)e.y;
         }
+        fin_values<T, D>(a, r, key, col, v);
 #pragma unroll
         for (int f = 0; f < FLIGHT; ++f)
           if (i0 + f * SIDE < m) {
@@ -441,8 +671,8 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
         for (int j = 0; j < EPL; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
       if (lane < LPR)
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) write(col + j, acc[j]);
-      if (lane == 0) write_tau(tau);
+        for (int j = 0; j < EPL; ++j) out[col + j] = from_float<T>(acc[j]);
+      if (lane == 0 && tau_out) *tau_out = tau;
     }
   }
 
@@ -451,110 +681,8 @@ __global__ void __launch_bounds__(kFinThreads, 3) tree_finish_kernel(const __gri
   for (int w = 0; w < kFinWarps; ++w) {
     if (!s_heavy[w]) continue;                   // uniform over the block
     __syncthreads();                             // the slots are free
-    r = fin_row(a, id0 + w, lane);
-    const float* const zd_w = reinterpret_cast<const float*>(s_dyn + n_ends) + w * a.tokens;
-    int all = 0;
-    float floor_w = -INFINITY;
-    if (a.dense) {                               // nothing bounds tau yet: the maximum first
-      all = r.len;
-      const float* const z = reinterpret_cast<const float*>(r.region) + a.region;
-      for (int i = tid; i < all; i += kFinThreads) floor_w = max_nan(floor_w, z[i]);
-      for (int j = tid; j < a.tokens; j += kFinThreads) floor_w = max_nan(floor_w, zd_w[j]);
-      floor_w = warp_max_nan(floor_w);
-      if (lane == 0) scratch[warp] = floor_w;
-      __syncthreads();
-#pragma unroll
-      for (int v = 0; v < kFinWarps; ++v) floor_w = max_nan(floor_w, scratch[v]);
-      floor_w -= 1.f;
-      __syncthreads();
-    } else {
-      const int* const counts = a.counts + r.id * a.max_parts * a.sub;
-      const float* const bounds = a.bounds + r.id * a.max_parts * a.sub;
-      for (int i0 = 0; i0 < r.lists; i0 += kFinThreads) {
-        const bool in = i0 + tid < r.lists;
-        const int c = in ? counts[i0 + tid] : 0;
-        if (in) floor_w = fmaxf(floor_w, bounds[i0 + tid]);
-        int total;
-        const int before = block_excl(c, reinterpret_cast<int*>(scratch), &total);
-        if (in) s_dyn[i0 + tid] = fin_list(a, r, i0 + tid, all + before, c);
-        all += total;
-      }
-      floor_w = block_max(floor_w, scratch);
-      __syncthreads();
-    }
-    const FinHeavy rows{s_slots, r.region};
-    // what the largest bound leaves, in order; a NaN stays
-    n = 0;
-    top = -INFINITY;
-    for (int i0 = 0; i0 < all + a.tokens; i0 += kFinThreads) {
-      const int i = i0 + tid;
-      uint2 e = make_uint2(__float_as_uint(-INFINITY), 0);
-      if (i < all) e = fin_entry(a, r, s_dyn, i);
-      else if (i < all + a.tokens) e = make_uint2(__float_as_uint(zd_w[i - all]), (uint32_t)~(i - all));
-      const bool keep = i < all + a.tokens && !(__uint_as_float(e.x) <= floor_w);
-      if (keep) top = max_nan(top, __uint_as_float(e.x));
-      int total;
-      const int at = n + block_excl(keep, reinterpret_cast<int*>(scratch), &total);
-      if (keep) rows.put(at, e);
-      n += total;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    __syncthreads();
-    if (lane == 0) scratch[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kFinWarps; ++v) top = max_nan(top, scratch[v]);
-    if (!(fabsf(top) < INFINITY)) {
-      const float fill = top == -INFINITY ? 0.f : NAN;
-      if (tid < D) write(tid, fill);
-      if (tid == 0) write_tau(top == -INFINITY ? INFINITY : NAN);
-      continue;
-    }
-    const float tau = fin_tau(fmaxf(floor_w, top - 1.f), top, a.alpha, kind, [&](float t) {
-      float2 s = make_float2(0.f, 0.f);
-      float s2 = 0.f;
-      for (int i = tid; i < n; i += kFinThreads)
-        halley_accumulate(__uint_as_float(rows.get(i).x), t, kind, beta, s.x, s.y, s2);
-      return block_sum2(s, scratch);
-    });
-    int m = 0;
-    for (int i0 = 0; i0 < n; i0 += kFinThreads) {
-      const int i = i0 + tid;
-      uint2 e = make_uint2(0, 0);
-      float weight = 0.f;
-      if (i < n) {
-        e = rows.get(i);
-        weight = entmax_weight(__uint_as_float(e.x), tau, kind, beta);
-      }
-      int total;
-      const int at = m + block_excl(weight > 0.f, reinterpret_cast<int*>(scratch), &total);
-      if (weight > 0.f) rows.put(at, make_uint2(__float_as_uint(weight), e.y));
-      m += total;
-    }
-    __syncthreads();
-    float acc[EPL] = {};
-    const int sub = tid / LPR, col = tid % LPR * EPL;
-#pragma unroll 4
-    for (int i = sub; i < m; i += GROUPS) {
-      const uint2 e = rows.get(i);
-      float x[EPL];
-      unpack<T>(fin_value<T, D>(a, r, (int)e.y, col), x);
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) acc[j] = fmaf(__uint_as_float(e.x), x[j], acc[j]);
-    }
-    __syncthreads();                             // the slots become partial sums
-    float* const s_acc = reinterpret_cast<float*>(s_slots);
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) s_acc[sub * D + col + j] = acc[j];
-    __syncthreads();
-    if (tid < D) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < GROUPS; ++i) s += s_acc[i * D + tid];
-      write(tid, s);
-    }
-    if (tid == 0) write_tau(tau);
+    fin_block_row<T, D, kFinWarps>(a, fin_row(a, id0 + w, lane), s_slots, s_lists,
+                                   reinterpret_cast<const float*>(s_lists + n_lists) + w * a.tokens, scratch);
   }
 }
 
@@ -699,7 +827,8 @@ static int launch_scores(const TreeArgs& a, const TreePlan& p, const CUtensorMap
 static bool tree_sizes_ok(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
   return q_heads > 0 && q_heads % c->kv_heads == 0 && tokens > 0 && tokens <= EKV_TREE_MAX_TOKENS && max_seq >= 0 &&
          max_seq <= c->capacity && max_seq <= c->page_capacity * (int64_t)c->page_size &&
-         (int64_t)tokens * (q_heads / c->kv_heads) <= (1 << 20) && (int64_t)c->batch * q_heads * tokens <= 0x7fffffff;
+         (int64_t)tokens * (q_heads / c->kv_heads) <= (1 << 20) && (int64_t)c->batch * q_heads * tokens <= 0x7fffffff &&
+         (!c->block_table || (int64_t)c->num_blocks * c->page_size <= 0x7fffffff);
 }
 
 unsigned int copy_timeouts_tree() { return copy_timeouts_here(); }
@@ -777,8 +906,10 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   a.list_cols = p.list_cols;
   a.sample_tiles = p.sample_tiles;
   a.tile_keys = p.tile_keys;
-  const int n_ends = fin_ends(p.max_parts * p.sub);
-  const size_t fin_smem = sizeof(uint2) * ((size_t)kFinSlots + n_ends) + sizeof(float) * (size_t)kFinWarps * tokens;
+  // few rows: a block each, while those fit the GPU in about two waves (three of these blocks to an SM)
+  const bool one = (int64_t)groups * p.rows <= 6 * sm_count();
+  const int n_lists = one ? p.max_parts * p.sub : fin_lists(p.max_parts * p.sub);
+  const size_t fin_smem = sizeof(uint2) * ((size_t)kFinSlots + n_lists) + sizeof(float) * (size_t)(one ? 1 : kFinWarps) * tokens;
   cudaStream_t st = as_stream(stream);
   CUtensorMap k_map{};
   if (p.mma && max_seq_len > 0)
@@ -792,11 +923,13 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
     EKV_DISPATCH(c->dtype, c->head_dim, {
       if (max_seq_len > 0) err = launch_scores<T, D>(a, p, k_map, st);
       if (err) return err;
-      cudaError_t e = cudaFuncSetAttribute(tree_finish_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)fin_smem);
-      if (e == cudaSuccess)
-        e = launch_after(tree_finish_kernel<T, D>, (unsigned)((rows + kFinWarps - 1) / kFinWarps), kFinThreads, fin_smem,
-                         st, max_seq_len > 0, a, rows, n_ends);
+      const auto finish = [&](auto kernel, unsigned grid, int threads, auto... args) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fin_smem);
+        return e != cudaSuccess ? e : launch_after(kernel, grid, threads, fin_smem, st, max_seq_len > 0, a, args...);
+      };
+      const cudaError_t e = one ? finish(tree_finish_one_kernel<T, D>, (unsigned)rows, kFinOneWarps * 32, n_lists)
+                                : finish(tree_finish_kernel<T, D>, (unsigned)((rows + kFinWarps - 1) / kFinWarps),
+                                         kFinWarps * 32, rows, n_lists);
       if (e != cudaSuccess) return (int)e;
     });
   }

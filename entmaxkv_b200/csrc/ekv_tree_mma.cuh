@@ -157,9 +157,9 @@ __global__ void __launch_bounds__(256) tree_bounds_kernel(const __grid_constant_
   const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   tree_let_next_start();
   if (id >= n_rows) return;
-  const int b = (a.g0 + (int)(id / a.rows)) / a.c.kv_heads;
+  const int gl = (int)((unsigned)id / (unsigned)a.rows), b = (a.g0 + gl) / a.c.kv_heads;
   const int n = tree_tiles<true>(a, b) * 4;
-  const bool live = (a.row0 + (int)(id % a.rows)) / a.group < tree_drafts(a, b);
+  const bool live = (a.row0 + (int)id - gl * a.rows) / a.group < tree_drafts(a, b);
   tree_wait_for_previous();
   if (!live || n == 0) return;
   const float* const cls = a.classes + id * a.sample_tiles * 4;
