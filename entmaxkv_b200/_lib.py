@@ -153,6 +153,8 @@ def ptr(t) -> int | None:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+#: index of the current device; torch's own accessor without its Python layers where it exists
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def stream_ptr() -> int:
@@ -160,7 +162,7 @@ def stream_ptr() -> int:
     accessor when it exists: building a ``torch.cuda.Stream`` object costs ~6 us per call, a seventh of the host
     time of a whole eager decode step.)"""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -177,7 +179,7 @@ _here = _Here()
 
 def on_device(t: torch.Tensor):
     """Context in which the device of ``t`` is the current one: streams and launches belong to the current device."""
-    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _here if t.get_device() == current_device() else torch.cuda.device(t.device)
 
 
 def require_cuda(*tensors) -> None:
@@ -187,6 +189,7 @@ def require_cuda(*tensors) -> None:
 
 
 def require_same_device(device, *tensors) -> None:
+    index = device.index
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"all tensors must be on {device}; got one on {t.device}")

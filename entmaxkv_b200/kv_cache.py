@@ -61,6 +61,7 @@ class PagedKVCache:
         self._meta = None                      # [4, B, H, page_capacity, D]: min, max, mean, std
         self.seq_lens: Optional[torch.Tensor] = None     # int32 [B] on the device
         self._host_lens: list[int] = []
+        self._longest = (None, 0)              # (a _host_lens, its largest)
         self._lens_exact = True                # False: device lengths may be below the host's
         self._may_be_empty = False             # True: a sequence may hold no token (released, or rewound to 0)
         self._ctl = None                       # int32: [0]=status, [16:16+B] append tickets
@@ -73,7 +74,9 @@ class PagedKVCache:
     @property
     def seq_len(self) -> int:
         """Longest sequence of the batch (the reference's ``k_cache.shape[2]``)."""
-        return max(self._host_lens) if self._host_lens else 0
+        if self._longest[0] is not self._host_lens:      # the list is replaced whenever a length changes
+            self._longest = (self._host_lens, max(self._host_lens) if self._host_lens else 0)
+        return self._longest[1]
 
     @property
     def host_seq_lens(self) -> list[int]:
@@ -341,10 +344,10 @@ class PagedKVCache:
             raise ValueError(f"index must be int32 [{B}, {T}], contiguous along the tokens")
         counts_host, counts = self._row_lens(counts, "counts", T)
         start_host, start = self._row_lens(start, "start", None)
-        bound = [min(s, n) if start_host is not None else n for s, n in zip(start_host or self._host_lens, self._host_lens)]
-        bound = [n + m for n, m in zip(bound, counts_host or [T] * B)]
-        if max_seq_len is not None:
-            bound = [min(n, max_seq_len) for n in bound]
+        bound = self._host_lens if start_host is None else [min(s, n) for s, n in zip(start_host, self._host_lens)]
+        bound = [n + T for n in bound] if counts_host is None else [n + m for n, m in zip(bound, counts_host)]
+        if max_seq_len is not None and max(bound) > max_seq_len:
+            bound = [n if n < max_seq_len else max_seq_len for n in bound]
         rewound_on_device = start is not None and start_host is None
         if T == 0:
             if start is None:
@@ -380,8 +383,9 @@ class PagedKVCache:
 
     def _make_room(self, lens):
         """Before tokens are added: room for sequences of ``lens`` tokens (upper bounds), and blocks in a shared pool."""
-        if max(lens) > self.capacity:
-            self.reserve(max(max(lens), self.capacity + 4096, self.capacity * 5 // 4))
+        most = max(lens)
+        if most > self.capacity:
+            self.reserve(max(most, self.capacity + 4096, self.capacity * 5 // 4))
         if self.num_blocks is not None and sum(-(-n // self.page_size) for n in lens) > self.num_blocks:
             raise RuntimeError(f"the pool of {self.num_blocks} blocks may not suffice: release() sequences" + (
                 "" if self._lens_exact else ", or call sync_lengths() (the host knows only upper bounds of the lengths)"))

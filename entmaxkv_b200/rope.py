@@ -13,21 +13,28 @@ import torch
 
 from . import _lib
 
-_STRIDES = C.c_int64 * 3
+_STRIDES = [C.c_int64 * (3 * n) for n in range(5)]
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself when its rows are 16-byte aligned and contiguous, else a copy."""
     e = t.element_size()
     s = t.stride()
-    if s[3] != 1 or t.data_ptr() % 16 or s[0] * e % 16 or s[1] * e % 16 or s[2] * e % 16:
+    if s[3] != 1 or (s[0] | s[1] | s[2]) * e % 16 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
+def _strides(*tensors):
+    """Batch, head and token strides of the tensors in one ctypes array, and the address of each one's three."""
+    array = _STRIDES[len(tensors)](*[x for t in tensors for x in t.stride()[:3]])
+    base = C.addressof(array)
+    return array, [base + 24 * i for i in range(len(tensors))]
+
+
 def _destination(out, like, name):
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must match its input in shape, dtype and device")
     if out.numel() and (_rows(out) is not out or any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride()))):
@@ -77,10 +84,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     with _lib.on_device(q):
         q_out, k_out = _destination(q_out, q, "q_out"), _destination(k_out, k, "k_out")
         q, k = _rows(q), _rows(k)
+        array, (qs, ks, qos, kos) = _strides(q, k, q_out, k_out)
         _lib.check(_lib.load().ekv_qk_norm_rope(
-            code, B, T, Hq, k.shape[1], D, q.data_ptr(), _STRIDES(*q.stride()[:3]), k.data_ptr(),
-            _STRIDES(*k.stride()[:3]), q_out.data_ptr(), _STRIDES(*q_out.stride()[:3]), k_out.data_ptr(),
-            _STRIDES(*k_out.stride()[:3]), positions.data_ptr(), int(positions.dtype == torch.int64),
+            code, B, T, Hq, k.shape[1], D, q.data_ptr(), qs, k.data_ptr(), ks, q_out.data_ptr(), qos,
+            k_out.data_ptr(), kos, positions.data_ptr(), int(positions.dtype == torch.int64),
             positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1), inv_freq.data_ptr(), half,
             int(interleaved), _lib.ptr(q_weight), _lib.ptr(k_weight), weight_f32, int(eps is not None),
             0.0 if eps is None else eps, _lib.stream_ptr()), "ekv_qk_norm_rope")

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .kv_cache import PagedKVCache
-from .rope import _STRIDES, _rows
+from .rope import _rows, _strides
 
 #: drafted tokens per sequence
 MAX_TOKENS = 256
@@ -75,10 +75,11 @@ def tree_attention_decode(q: torch.Tensor, kv_cache: PagedKVCache, k_draft: torc
         desc = C.byref(kv_cache.desc())
         # scratch of this call alone, from torch's stream-ordered allocator: two streams or two graphs never share it
         ws = torch.empty(lib.ekv_tree_workspace_bytes(desc, Hq, T, bound), dtype=torch.uint8, device=device)
+        array, (qs, ks, vs, os_) = _strides(q, k_draft, v_draft, out)
+        ms = tree_mask.stride()
         _lib.check(lib.ekv_tree_decode(
-            desc, q.data_ptr(), _STRIDES(*q.stride()[:3]), Hq, T, k_draft.data_ptr(), _STRIDES(*k_draft.stride()[:3]),
-            v_draft.data_ptr(), _STRIDES(*v_draft.stride()[:3]), tree_mask.data_ptr(),
-            tree_mask.stride(0) if tree_mask.dim() == 3 else 0, tree_mask.stride(-2), _lib.ptr(draft_lens), bound,
-            float(alpha), out.data_ptr(), _STRIDES(*out.stride()[:3]), _lib.ptr(taus_out), ws.data_ptr(), ws.numel(),
+            desc, q.data_ptr(), qs, Hq, T, k_draft.data_ptr(), ks, v_draft.data_ptr(), vs, tree_mask.data_ptr(),
+            ms[0] if len(ms) == 3 else 0, ms[-2], _lib.ptr(draft_lens), bound, float(alpha), out.data_ptr(), os_,
+            _lib.ptr(taus_out), ws.data_ptr(), ws.numel(),
             kv_cache._ctl.data_ptr(), _lib.stream_ptr()), "ekv_tree_decode")
     return out
