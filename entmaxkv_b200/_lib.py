@@ -177,9 +177,9 @@ class _Here:
 _here = _Here()
 
 
-def on_device(t: torch.Tensor):
-    """Context in which the device of ``t`` is the current one: streams and launches belong to the current device."""
-    return _here if t.get_device() == current_device() else torch.cuda.device(t.device)
+def on_device(index: int):
+    """Context in which device ``index`` is the current one: streams and launches belong to the current device."""
+    return _here if index == current_device() else torch.cuda.device(index)
 
 
 def require_cuda(*tensors) -> None:
@@ -188,8 +188,12 @@ def require_cuda(*tensors) -> None:
             raise ValueError("entmaxkv_b200 runs on CUDA tensors only (sm_100a); got a CPU tensor")
 
 
-def require_same_device(device, *tensors) -> None:
-    index = device.index
+def require_on_one_device(first, *tensors) -> int:
+    """All tensors (None: left out) are on the CUDA device of ``first``, whose index is returned."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError("entmaxkv_b200 runs on CUDA tensors only (sm_100a); got a CPU tensor")
     for t in tensors:
         if t is not None and t.get_device() != index:
-            raise ValueError(f"all tensors must be on {device}; got one on {t.device}")
+            raise ValueError(f"all tensors must be CUDA tensors on {first.device}; got one on {t.device}")
+    return index

@@ -16,29 +16,30 @@ from . import _lib
 MAX_BATCH = 16384
 
 
-def _check(seq_lens, other, block_table, free_blocks, page_size, name):
-    _lib.require_cuda(seq_lens, block_table, free_blocks)
-    B = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    if seq_lens.dtype != torch.int32 or B < 0 or not seq_lens.is_contiguous():
+def _check(seq_lens, other, block_table, free_blocks, page_size, name, *outputs):
+    """(B, device index, other is a tensor) of arguments that hold together."""
+    per_row = isinstance(other, torch.Tensor)
+    index = _lib.require_on_one_device(seq_lens, other if per_row else None, block_table, free_blocks, *outputs)
+    shape, table = seq_lens.shape, block_table.shape
+    if seq_lens.dtype != torch.int32 or len(shape) != 1 or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be a contiguous int32 [B] tensor")
+    B = shape[0]
     if B > MAX_BATCH:
         raise ValueError(f"at most {MAX_BATCH} sequences per call")
-    if isinstance(other, torch.Tensor):
-        _lib.require_same_device(seq_lens.device, other)
-        if other.dtype != torch.int32 or tuple(other.shape) != (B,) or not other.is_contiguous():
+    if per_row:
+        if other.dtype != torch.int32 or other.shape != shape or not other.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 [B] tensor or an int")
     elif isinstance(other, bool) or not isinstance(other, int) or not 0 <= other < 1 << 31:
         raise ValueError(f"{name} must be a contiguous int32 [B] tensor or an int >= 0")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1) or (
-            B > 1 and block_table.stride(0) < block_table.shape[1]):
+    if block_table.dtype != torch.int32 or len(table) != 2 or table[0] != B or (
+            not block_table.is_contiguous() and ((table[1] > 1 and block_table.stride(1) != 1)
+                                                 or (B > 1 and block_table.stride(0) < table[1]))):
         raise ValueError("block_table must be int32 [B, pages], contiguous along the pages")
     if free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
         raise ValueError("free_blocks must be a contiguous int32 [num_blocks] tensor")
     if page_size <= 0:
         raise ValueError("page_size must be positive")
-    _lib.require_same_device(seq_lens.device, block_table, free_blocks)
-    return B
+    return B, index, per_row
 
 
 def plan_block_tables(seq_lens: torch.Tensor, new_lens: Union[torch.Tensor, int], block_table: torch.Tensor,
@@ -58,28 +59,30 @@ def plan_block_tables(seq_lens: torch.Tensor, new_lens: Union[torch.Tensor, int]
     ``seq_lens`` has grown.  ``status`` (int32, optional) gets bit 2 (capacity) when the pool or the table did not
     suffice.  Returns (block_table, slots, positions, row_starts).
     """
-    B = _check(seq_lens, new_lens, block_table, free_blocks, page_size, "new_lens")
+    B, index, per_row = _check(seq_lens, new_lens, block_table, free_blocks, page_size, "new_lens", slots, positions,
+                               row_starts, status)
     n = 0
-    for t, dt in ((slots, torch.int64), (positions, torch.int32)):
-        if t is not None:
-            if t.dtype != dt or t.dim() != 1 or not t.is_contiguous() or (n and t.shape[0] != n):
-                raise ValueError("slots (int64) and positions (int32) must be contiguous, one entry per token")
-            n = t.shape[0]
-    if slots is not None and positions is not None and slots.shape != positions.shape:
-        raise ValueError("slots (int64) and positions (int32) must be contiguous, one entry per token")
-    if row_starts is not None and (row_starts.dtype != torch.int32 or tuple(row_starts.shape) != (B + 1,)
+    if slots is not None:
+        n = slots.shape[0] if slots.dim() == 1 else -1
+        if slots.dtype != torch.int64 or n < 0 or not slots.is_contiguous():
+            raise ValueError("slots must be contiguous int64, one entry per token")
+    if positions is not None:
+        m = positions.shape[0] if positions.dim() == 1 else -1
+        if positions.dtype != torch.int32 or m < 0 or not positions.is_contiguous() or (slots is not None and m != n):
+            raise ValueError("positions must be contiguous int32, one entry per token, as many as slots")
+        n = m
+    if row_starts is not None and (row_starts.dtype != torch.int32 or row_starts.shape != (B + 1,)
                                    or not row_starts.is_contiguous()):
         raise ValueError("row_starts must be a contiguous int32 [B + 1] tensor")
     if status is not None and status.dtype != torch.int32:
         raise ValueError("status must be int32")
-    _lib.require_same_device(seq_lens.device, slots, positions, row_starts, status)
-    with _lib.on_device(seq_lens):
-        per_row = isinstance(new_lens, torch.Tensor)
+    width = block_table.shape[1]
+    with _lib.on_device(index):
         _lib.check(_lib.load().ekv_plan_block_tables(
             seq_lens.data_ptr(), new_lens.data_ptr() if per_row else None, 0 if per_row else new_lens, B, page_size,
-            block_table.data_ptr(), block_table.stride(0) if B > 1 else block_table.shape[1], block_table.shape[1],
-            free_blocks.data_ptr(), free_blocks.shape[0], _lib.ptr(slots), _lib.ptr(positions), n,
-            _lib.ptr(row_starts), _lib.ptr(status), _lib.stream_ptr()), "ekv_plan_block_tables")
+            block_table.data_ptr(), block_table.stride(0) if B > 1 else width, width, free_blocks.data_ptr(),
+            free_blocks.shape[0], _lib.ptr(slots), _lib.ptr(positions), n, _lib.ptr(row_starts), _lib.ptr(status),
+            _lib.stream_ptr()), "ekv_plan_block_tables")
     return block_table, slots, positions, row_starts
 
 
@@ -88,7 +91,7 @@ def release_block_tables(seq_lens: torch.Tensor, keep_lens: Union[torch.Tensor, 
     """Return the pages behind the first ``keep_lens[b]`` tokens of every sequence to ``free_blocks`` and lower
     ``seq_lens`` to ``keep_lens`` (arguments as ``plan_block_tables``); their table entries become -1."""
     return_blocks(seq_lens, keep_lens, block_table, free_blocks, page_size, status)
-    with _lib.on_device(seq_lens):
+    with _lib.on_device(seq_lens.get_device()):
         if isinstance(keep_lens, torch.Tensor):
             torch.minimum(seq_lens, keep_lens.clamp(min=0), out=seq_lens)
         else:
@@ -98,13 +101,12 @@ def release_block_tables(seq_lens: torch.Tensor, keep_lens: Union[torch.Tensor, 
 
 def return_blocks(seq_lens, keep_lens, block_table, free_blocks, page_size, status=None) -> None:
     """``release_block_tables`` without lowering the lengths."""
-    B = _check(seq_lens, keep_lens, block_table, free_blocks, page_size, "keep_lens")
+    B, index, per_row = _check(seq_lens, keep_lens, block_table, free_blocks, page_size, "keep_lens", status)
     if status is not None and status.dtype != torch.int32:
         raise ValueError("status must be int32")
-    _lib.require_same_device(seq_lens.device, status)
-    with _lib.on_device(seq_lens):
-        per_row = isinstance(keep_lens, torch.Tensor)
+    width = block_table.shape[1]
+    with _lib.on_device(index):
         _lib.check(_lib.load().ekv_release_blocks(
             seq_lens.data_ptr(), keep_lens.data_ptr() if per_row else None, 0 if per_row else keep_lens, B, page_size,
-            block_table.data_ptr(), block_table.stride(0) if B > 1 else block_table.shape[1], block_table.shape[1],
-            free_blocks.data_ptr(), free_blocks.shape[0], _lib.ptr(status), _lib.stream_ptr()), "ekv_release_blocks")
+            block_table.data_ptr(), block_table.stride(0) if B > 1 else width, width, free_blocks.data_ptr(),
+            free_blocks.shape[0], _lib.ptr(status), _lib.stream_ptr()), "ekv_release_blocks")

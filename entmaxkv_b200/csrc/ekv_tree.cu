@@ -854,7 +854,7 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   if (!q || !q_strides || !k_draft || !k_strides || !v_draft || !v_strides || !mask || !out || !out_strides || !workspace)
     return EKV_ERR_ARG;
   if (!tree_sizes_ok(c, q_heads, tokens, max_seq_len)) return EKV_ERR_ARG;
-  if (!(alpha > 1.f)) return EKV_ERR_ALPHA;
+  if (!(alpha > 1.f) || !(alpha < INFINITY)) return EKV_ERR_ALPHA;
   const int64_t esz = c->dtype == EKV_F32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_draft) | reinterpret_cast<uintptr_t>(v_draft) |
        reinterpret_cast<uintptr_t>(workspace)) & 15)

@@ -63,6 +63,7 @@ class PagedKVCache:
         self._host_lens: list[int] = []
         self._longest = (None, 0)              # (a _host_lens, its largest)
         self._lens_exact = True                # False: device lengths may be below the host's
+        self._grows_in_graphs = False          # True: tokens are added by captured calls, whose replays the host does not see
         self._may_be_empty = False             # True: a sequence may hold no token (released, or rewound to 0)
         self._ctl = None                       # int32: [0]=status, [16:16+B] append tickets
         self.last_num_selected_per_head = None
@@ -107,7 +108,7 @@ class PagedKVCache:
             blocks = pool[self._table[:, :n].reshape(-1).long()]                 # [B*n, H, P, D]
             dense = blocks.view(B, n, H, self.page_size, D).permute(0, 2, 1, 3, 4).reshape(B, H, n * self.page_size, D)
             return dense[:, :, :self.seq_len]
-        return t[:, :, :self.seq_len]
+        return t.narrow(2, 0, self.seq_len)
 
     @property
     def k_cache(self):
@@ -118,7 +119,7 @@ class PagedKVCache:
         return self._view_rows(self._v, self._pool_v)
 
     def _meta_view(self, i):
-        return None if self._meta is None else self._meta[i][:, :, :self.num_pages]
+        return None if self._meta is None else self._meta.select(0, i).narrow(2, 0, self.num_pages)
 
     @property
     def k_min(self):
@@ -304,6 +305,7 @@ class PagedKVCache:
             self.extend(k_new, v_new)
             return
         self._make_room([n + 1 for n in self._host_lens])
+        self._grows_in_graphs |= torch.cuda.is_current_stream_capturing()
         lib = _lib.load()
         _lib.check(lib.ekv_append(C.byref(self.desc()), k_new.data_ptr(), v_new.data_ptr(),
                                   k_new.stride(0), k_new.stride(1),
@@ -324,22 +326,23 @@ class PagedKVCache:
         ``counts`` and ``start`` are sequences of ints, or int32 CUDA tensors.  The host does not read the latter, so
         its view of the lengths (``seq_len``, ``host_seq_lens``, the row range of ``k_cache``) becomes an upper bound:
         ``T`` more tokens for every sequence, or ``max_seq_len`` where that is given and smaller (rows past it are then
-        the caller's mistake).  ``sync_lengths`` makes it exact again.  Values out of range are clipped on the device and
-        show in ``device_status``.
+        the caller's mistake).  ``sync_lengths`` makes it exact again; call it after replays of a captured ``extend``, too,
+        which the host does not count.  Values out of range are clipped on the device and show in ``device_status``.
+        ``k_new`` and ``v_new`` must not be views of the cache itself.
         """
         if self._k is None:
             raise RuntimeError("initialize() the cache before extend()")
-        _lib.require_cuda(k_new, v_new)
+        dev = _lib.require_on_one_device(self._k, k_new, v_new, index)
         B, H, _, D = self._k.shape
-        if k_new.dim() != 4 or k_new.shape != v_new.shape or (k_new.shape[0], k_new.shape[1], k_new.shape[3]) != (B, H, D):
+        shape, dtype = k_new.shape, self._k.dtype
+        if len(shape) != 4 or v_new.shape != shape or (shape[0], shape[1], shape[3]) != (B, H, D):
             raise ValueError(f"k_new / v_new must be [{B}, {H}, T, {D}]")
-        if k_new.dtype != self._k.dtype or v_new.dtype != self._k.dtype:
+        if k_new.dtype != dtype or v_new.dtype != dtype:
             raise ValueError("k_new / v_new dtype differs from the cache dtype")
-        device, T = self._k.device, k_new.shape[2]
-        _lib.require_same_device(device, k_new, v_new, index)
+        device, T = self._k.device, shape[2]
         if max_seq_len is not None and max_seq_len < 0:
             raise ValueError("max_seq_len must be >= 0")
-        if index is not None and (index.dtype != torch.int32 or tuple(index.shape) != (B, T)
+        if index is not None and (index.dtype != torch.int32 or index.shape != (B, T)
                                   or (T > 1 and index.stride(1) != 1)):
             raise ValueError(f"index must be int32 [{B}, {T}], contiguous along the tokens")
         counts_host, counts = self._row_lens(counts, "counts", T)
@@ -356,12 +359,12 @@ class PagedKVCache:
             counts, T, index = torch.zeros(B, dtype=torch.int32, device=device), 1, None
         e = k_new.element_size()
         s = k_new.stride()
-        if (s != v_new.stride() or s[3] != 1 or s[0] * e % 16 or s[1] * e % 16 or s[2] * e % 16
-                or (k_new.data_ptr() | v_new.data_ptr()) % 16):
+        if s != v_new.stride() or s[3] != 1 or (s[0] | s[1] | s[2]) * e % 16 or (k_new.data_ptr() | v_new.data_ptr()) % 16:
             k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
             s = k_new.stride()
-        with _lib.on_device(k_new):
+        with _lib.on_device(dev):
             self._make_room(bound)
+            self._grows_in_graphs |= torch.cuda.is_current_stream_capturing()
             if self.num_blocks is not None:
                 held = self.seq_lens
                 if start is not None:          # what lies behind the rewind goes back first
@@ -372,7 +375,7 @@ class PagedKVCache:
             _lib.check(_lib.load().ekv_extend(
                 C.byref(self.desc()), k_new.data_ptr(), v_new.data_ptr(), s[0], s[1], s[2], T, _lib.ptr(counts),
                 _lib.ptr(index), index.stride(0) if index is not None and B > 1 else T, _lib.ptr(start),
-                self._ctl[16:].data_ptr(), self._ctl.data_ptr(), _lib.stream_ptr()), "ekv_extend")
+                self._ctl.data_ptr() + 64, self._ctl.data_ptr(), _lib.stream_ptr()), "ekv_extend")
         if counts_host is None or rewound_on_device:
             self._lens_exact = False
         if counts_host is not None and min(counts_host) > 0:
@@ -396,9 +399,8 @@ class PagedKVCache:
         if value is None:
             return ([most] * B if most is not None else None), None
         if isinstance(value, torch.Tensor):
-            _lib.require_cuda(value)
-            _lib.require_same_device(device, value)
-            if value.dtype != torch.int32 or tuple(value.shape) != (B,) or not value.is_contiguous():
+            _lib.require_on_one_device(self._k, value)
+            if value.dtype != torch.int32 or value.shape != (B,) or not value.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous int32 [{B}] tensor")
             return None, value
         host = [int(x) for x in value]

@@ -13,6 +13,7 @@ import torch
 
 from . import _lib
 
+_INTS = (torch.int32, torch.int64)
 _STRIDES = [C.c_int64 * (3 * n) for n in range(5)]
 
 
@@ -55,14 +56,17 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     of 8 entries, at most D / 2; weights: [D], both in the tensors' dtype or both fp32.  ``q_out`` / ``k_out`` may be
     the inputs themselves (in place) and must not overlap them otherwise.  Returns (q_out, k_out).
     """
-    _lib.require_cuda(q, k, positions, inv_freq, q_weight, k_weight)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+    index = _lib.require_on_one_device(q, k, positions, inv_freq, q_weight, k_weight)
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 4 or len(k_shape) != 4 or (q_shape[0], q_shape[2], q_shape[3]) != (k_shape[0], k_shape[2], k_shape[3]):
         raise ValueError("q must be [B, H_q, T, D] and k [B, H_kv, T, D]")
-    B, Hq, T, D = q.shape
-    if q.dtype != k.dtype:
+    B, Hq, T, D = q_shape
+    dtype = q.dtype
+    if k.dtype != dtype:
         raise ValueError("q and k must have one dtype")
-    code = _lib.dtype_code(q.dtype)
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((B, T), (T,)):
+    code = _lib.dtype_code(dtype)
+    p_dtype, p_shape, p_strides = positions.dtype, positions.shape, positions.stride()
+    if p_dtype not in _INTS or not (p_shape == (B, T) or p_shape == (T,)):
         raise ValueError(f"positions must be int32 or int64, [{B}, {T}] or [{T}]")
     half = inv_freq.shape[0] if inv_freq.dim() == 1 else -1
     if half < 0 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or half % 8 or 2 * half > D:
@@ -72,23 +76,21 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
         if eps is None:
             raise ValueError("weights belong to the norm; eps=None switches it off")
         for w in (q_weight, k_weight):
-            if w is not None and (tuple(w.shape) != (D,) or w.dtype not in (q.dtype, torch.float32)
-                                  or not w.is_contiguous()):
+            if w is not None and (w.shape != (D,) or w.dtype not in (dtype, torch.float32) or not w.is_contiguous()):
                 raise ValueError(f"weights must be contiguous [{D}] tensors in the dtype of q or fp32")
         if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
             raise ValueError("q_weight and k_weight must have one dtype")
         weight_f32 = int((k_weight if q_weight is None else q_weight).dtype == torch.float32)
     if eps is not None and not eps >= 0:
         raise ValueError("eps must be >= 0 (or None)")
-    _lib.require_same_device(q.device, k, positions, inv_freq, q_weight, k_weight)
-    with _lib.on_device(q):
+    with _lib.on_device(index):
         q_out, k_out = _destination(q_out, q, "q_out"), _destination(k_out, k, "k_out")
         q, k = _rows(q), _rows(k)
         array, (qs, ks, qos, kos) = _strides(q, k, q_out, k_out)
         _lib.check(_lib.load().ekv_qk_norm_rope(
-            code, B, T, Hq, k.shape[1], D, q.data_ptr(), qs, k.data_ptr(), ks, q_out.data_ptr(), qos,
-            k_out.data_ptr(), kos, positions.data_ptr(), int(positions.dtype == torch.int64),
-            positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1), inv_freq.data_ptr(), half,
+            code, B, T, Hq, k_shape[1], D, q.data_ptr(), qs, k.data_ptr(), ks, q_out.data_ptr(), qos,
+            k_out.data_ptr(), kos, positions.data_ptr(), int(p_dtype == torch.int64),
+            p_strides[0] if len(p_strides) == 2 else 0, p_strides[-1], inv_freq.data_ptr(), half,
             int(interleaved), _lib.ptr(q_weight), _lib.ptr(k_weight), weight_f32, int(eps is not None),
             0.0 if eps is None else eps, _lib.stream_ptr()), "ekv_qk_norm_rope")
     return q_out, k_out

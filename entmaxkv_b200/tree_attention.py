@@ -8,6 +8,7 @@ keys and values stay outside the cache; ``PagedKVCache.extend`` writes the accep
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional
 
 import torch
@@ -33,53 +34,57 @@ def tree_attention_decode(q: torch.Tensor, kv_cache: PagedKVCache, k_draft: torc
     ``p = ((alpha-1) q.k / sqrt(D) - tau)_+^(1/(alpha-1))`` with the tau that makes each row sum to one, solved until it
     no longer moves; ``out = sum p v``, written in place and returned.  A row that sees nothing gets zeros and
     ``tau = +inf``; a NaN or infinite score makes its row NaN.  ``taus_out`` (fp32 [B, H_q, T], contiguous) receives the
-    thresholds.  Works on dense and block-table caches; the cache is not changed.
+    thresholds.  Works on dense and block-table caches; the cache is not changed.  ``out`` must not overlap the inputs.
+    Scratch comes from torch's allocator, about 8 bytes per row and cached token up to 6 GiB, of which little is touched.
     """
     if kv_cache._k is None:
         raise RuntimeError("kv_cache is not initialised")
-    if not alpha > 1.0:
-        raise ValueError("alpha must be > 1")
-    _lib.require_cuda(q, k_draft, v_draft, tree_mask, out, draft_lens, taus_out)
+    if not 1.0 < alpha < math.inf:
+        raise ValueError("alpha must be > 1 and finite")
+    index = _lib.require_on_one_device(kv_cache._k, q, k_draft, v_draft, tree_mask, out, draft_lens, taus_out)
     B, Hkv, _, D = kv_cache._k.shape
-    dtype, device = kv_cache._k.dtype, kv_cache._k.device
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[1] == 0 or q.shape[1] % Hkv:
+    dtype, shape = kv_cache._k.dtype, q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != D or shape[1] == 0 or shape[1] % Hkv:
         raise ValueError(f"q must be [{B}, H_q, T, {D}] with H_q a multiple of {Hkv}")
-    Hq, T = q.shape[1], q.shape[2]
+    Hq, T = shape[1], shape[2]
     if T > MAX_TOKENS:
         raise ValueError(f"at most {MAX_TOKENS} drafted tokens per sequence")
-    if tuple(k_draft.shape) != (B, Hkv, T, D) or tuple(v_draft.shape) != (B, Hkv, T, D):
+    if k_draft.shape != (B, Hkv, T, D) or v_draft.shape != (B, Hkv, T, D):
         raise ValueError(f"k_draft / v_draft must be [{B}, {Hkv}, {T}, {D}]")
     if q.dtype != dtype or k_draft.dtype != dtype or v_draft.dtype != dtype or out.dtype != dtype:
         raise ValueError("q, k_draft, v_draft and out must have the cache's dtype")
-    if out.shape != q.shape or (T and out.stride(-1) != 1) or any(
-            n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+    if out.shape != shape or (not out.is_contiguous() and ((T and out.stride(-1) != 1) or any(
+            n > 1 and s == 0 for n, s in zip(shape, out.stride())))):
         raise ValueError("out must match q in shape and be contiguous along head_dim")
-    if tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((T, T), (B, T, T)) or (
-            T > 1 and tree_mask.stride(-1) != 1):
+    ms = tree_mask.stride()
+    if tree_mask.dtype != torch.bool or not (tree_mask.shape == (B, T, T) or tree_mask.shape == (T, T)) or (
+            T > 1 and ms[-1] != 1):
         raise ValueError(f"tree_mask must be bool [{T}, {T}] or [{B}, {T}, {T}], contiguous along its last axis")
-    if draft_lens is not None and (draft_lens.dtype != torch.int32 or tuple(draft_lens.shape) != (B,)
+    if draft_lens is not None and (draft_lens.dtype != torch.int32 or draft_lens.shape != (B,)
                                    or not draft_lens.is_contiguous()):
         raise ValueError(f"draft_lens must be a contiguous int32 [{B}] tensor")
-    if taus_out is not None and (tuple(taus_out.shape) != (B, Hq, T) or taus_out.dtype != torch.float32
+    if taus_out is not None and (taus_out.shape != (B, Hq, T) or taus_out.dtype != torch.float32
                                  or not taus_out.is_contiguous()):
         raise ValueError("taus_out must be a contiguous fp32 [B, H_q, T] tensor")
-    _lib.require_same_device(device, q, k_draft, v_draft, tree_mask, out, draft_lens, taus_out)
     if T == 0:
         return out
-    with _lib.on_device(q):
+    if out.data_ptr() in (q.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr()):
+        raise ValueError("out must not share memory with the inputs: rows are written while others still read them")
+    with _lib.on_device(index):
         lib = _lib.load()
         q, k_draft, v_draft = _rows(q), _rows(k_draft), _rows(v_draft)
-        # a captured call is replayed while the sequences grow: it is sized by the capacity
-        capturing = torch.cuda.is_current_stream_capturing()
-        bound = kv_cache.capacity if capturing else min(kv_cache.seq_len, kv_cache.capacity)
+        # a captured call is replayed while the sequences grow, and replayed appends grow them unseen by the host: then
+        # the call is sized by the capacity
+        unseen = kv_cache._grows_in_graphs or torch.cuda.is_current_stream_capturing()
+        bound = kv_cache.capacity if unseen else min(kv_cache.seq_len, kv_cache.capacity)
         desc = C.byref(kv_cache.desc())
         # scratch of this call alone, from torch's stream-ordered allocator: two streams or two graphs never share it
-        ws = torch.empty(lib.ekv_tree_workspace_bytes(desc, Hq, T, bound), dtype=torch.uint8, device=device)
+        ws_bytes = lib.ekv_tree_workspace_bytes(desc, Hq, T, bound)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
         array, (qs, ks, vs, os_) = _strides(q, k_draft, v_draft, out)
-        ms = tree_mask.stride()
         _lib.check(lib.ekv_tree_decode(
             desc, q.data_ptr(), qs, Hq, T, k_draft.data_ptr(), ks, v_draft.data_ptr(), vs, tree_mask.data_ptr(),
             ms[0] if len(ms) == 3 else 0, ms[-2], _lib.ptr(draft_lens), bound, float(alpha), out.data_ptr(), os_,
-            _lib.ptr(taus_out), ws.data_ptr(), ws.numel(),
+            _lib.ptr(taus_out), ws.data_ptr(), ws_bytes,
             kv_cache._ctl.data_ptr(), _lib.stream_ptr()), "ekv_tree_decode")
     return out

@@ -87,6 +87,75 @@ CASES = [
 ]
 
 
+# long enough for the sample and the candidate lists; row counts on both sides of a copy, a tile and a block of rows;
+# page sizes that are no multiple of eight, or do not divide a tile
+LONG = [
+    (1, 1, 1, 64, [9001], 1, 16, "bf16", 1.5, "dense", None),
+    (2, 4, 2, 128, [12289, 1], 9, 16, "bf16", 1.5, "pool", [9, 4]),
+    (1, 16, 1, 64, [8400], 2, 12, "fp16", 1.5, "pool", None),
+    (1, 8, 1, 128, [10007], 5, 1, "bf16", 2.0, "blocks", None),
+    (1, 5, 1, 128, [9500], 13, 200, "fp16", 1.5, "blocks", None),
+    (3, 4, 1, 64, [8193, 130, 20000], 20, 24, "bf16", 1.5, "pool", [20, 0, 11]),
+    (1, 8, 1, 64, [8300], 33, 16, "fp16", 2.0, "dense", None),      # 264 rows: two blocks of rows
+    (1, 4, 1, 128, [9100], 40, 16, "bf16", 1.5, "dense", None),     # 160 rows: two tiles of rows
+    (1, 2, 1, 64, [9000], 3, 16, "bf16", 4 / 3, "dense", None),
+    (1, 2, 1, 64, [9000], 3, 16, "fp16", 2.5, "pool", None),
+    (2, 32, 32, 64, [2600, 2500], 1, 16, "fp16", 1.5, "dense", None),   # short sequences, many heads
+    (40, 2, 2, 64, [2000 + 31 * i for i in range(40)], 2, 16, "bf16", 1.5, "dense", None),
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=[f"long{i}" for i in range(len(LONG))])
+def test_long_sequences_against_64_bits(case):
+    test_tree_attention_against_64_bits(case)
+
+
+def test_long_flat_scores():
+    """Every key a candidate of every row: the lists are full, and one block works on a row's lists in memory."""
+    for alpha, seed in ((1.5, 31), (2.0, 32)):
+        lens = [9100]
+        x = make(1, 4, 1, 64, lens, 2, torch.bfloat16, seed=seed, scale=1e-3)
+        out, tau = run(x, cache_of(x, lens, 16, "pool"), alpha)
+        check(x, lens, out, tau, alpha)
+
+
+def test_long_sequences_with_what_must_not_matter_and_what_must_show():
+    lens, T = [9000, 8700], 4
+    x = make(2, 4, 1, 64, lens, T, torch.float16, seed=33)
+    want = run(x, cache_of(x, lens, 16, "dense"), 1.5)
+    for _ in range(3):
+        got = run(x, cache_of(x, lens, 16, "pool"), 1.5)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    y = {n: t.clone() for n, t in x.items()}
+    y["k"][1, :, 8700:], y["v"][1, :, 8700:] = math.nan, math.nan
+    got = run(y, cache_of(y, lens, 16, "dense"), 1.5)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    y["k"][0, 0, 5000, 3] = math.nan
+    got = run(y, cache_of(y, lens, 16, "dense"), 1.5)
+    assert got[0][0].isnan().all() and torch.equal(got[0][1], want[0][1])
+
+
+def test_many_rows_share_the_scratch_in_turns():
+    """More rows than the scratch holds at a time: the same bits as sequence by sequence."""
+    import entmaxkv_b200 as E
+    B, Hq, Hkv, D, S, T = 2, 64, 8, 64, 131072, 56
+    g = torch.Generator(device="cuda").manual_seed(34)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    k, v, q, kd, vd = r(B, Hkv, S, D), r(B, Hkv, S, D), r(B, Hq, T, D), r(B, Hkv, T, D), r(B, Hkv, T, D)
+    mask = torch.ones(T, T, dtype=torch.bool, device="cuda").tril()
+    outs = []
+    for rows in (slice(0, 2), slice(0, 1), slice(1, 2)):
+        c = E.PagedKVCache(16, capacity=S)
+        c.initialize(k[rows], v[rows])
+        out = torch.zeros_like(q[rows])
+        E.tree_attention_decode(q[rows], c, kd[rows], vd[rows], mask, out)
+        outs.append(out)
+    # which scores a launch samples, and how it cuts the tiles, is another in each case: equal up to the summation order
+    both, each = outs[0].float(), torch.cat(outs[1:]).float()
+    assert (both - each).abs().max() <= 2 * 2.0 ** -8 * each.abs().max()
+    assert (both == each).float().mean() > 0.99
+
+
 @pytest.mark.parametrize("case", CASES, ids=[f"case{i}" for i in range(len(CASES))])
 def test_tree_attention_against_64_bits(case):
     B, Hq, Hkv, D, lens, T, page, dt, alpha, layout, drafts = case
@@ -190,10 +259,10 @@ def test_layouts_give_the_same_bits_and_runs_repeat():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
-def test_two_graphs_on_one_cache_and_a_growing_sequence():
+@pytest.mark.parametrize("lens", [[600, 300], [9000, 8500]])
+def test_two_graphs_on_one_cache_and_a_growing_sequence(lens):
     """Captured calls keep their scratch to themselves and follow the lengths on the device."""
     import entmaxkv_b200 as E
-    lens = [600, 300]
     x = make(2, 4, 2, 128, lens, 4, torch.bfloat16, seed=18)
     y = make(2, 4, 2, 128, lens, 9, torch.bfloat16, seed=19)
     cache = cache_of(x, lens, 16, "dense")
@@ -222,7 +291,9 @@ def test_two_graphs_on_one_cache_and_a_growing_sequence():
         for _, out, d in graphs:
             want = torch.zeros_like(out)
             E.tree_attention_decode(d["q"], cache, d["kd"], d["vd"], d["mask"], want)
-            assert torch.equal(out, want)
+            # the captured call is sized by the capacity: it may take the keys in another order
+            assert (out.float() - want.float()).abs().max() <= 2 * 2.0 ** -8 * want.float().abs().max()
+            assert (out == want).float().mean() > 0.99
 
 
 def test_refusals():
@@ -232,7 +303,7 @@ def test_refusals():
     out = torch.zeros_like(x["q"])
     good = dict(q=x["q"], kv_cache=cache, k_draft=x["kd"], v_draft=x["vd"], tree_mask=x["mask"], out=out)
     E.tree_attention_decode(**good)
-    bad = [dict(alpha=1.0), dict(alpha=math.nan), dict(q=x["q"][:, :3]), dict(q=x["q"].float()), dict(q=x["q"].cpu()),
+    bad = [dict(alpha=1.0), dict(alpha=math.nan), dict(alpha=math.inf), dict(out=x["q"]), dict(q=x["q"][:, :3]), dict(q=x["q"].float()), dict(q=x["q"].cpu()),
            dict(k_draft=x["kd"][:, :, :2]), dict(v_draft=x["vd"].float()), dict(tree_mask=x["mask"].int()),
            dict(tree_mask=x["mask"][:1]), dict(tree_mask=x["mask"].transpose(-1, -2)), dict(out=out[:, :, :2]),
            dict(out=out.float()), dict(out=out[:, :1].expand_as(out)),
