@@ -23,7 +23,7 @@ struct ExtendArgs {
   int* status;
 };
 
-constexpr int kExtendMaxThreads = 256;
+constexpr int kExtendMaxThreads = 128;
 constexpr int kExtendRows = 16;  // rows of a page held in registers at once
 
 // grid: (B * H_kv, page groups, 2: keys, values)

@@ -32,7 +32,7 @@ struct RopeArgs {
   int rows_per_block;
 };
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 constexpr int kRopeFlight = 4;      // rows of one thread whose loads are in flight together
 
 // two fp32 operations in one instruction
@@ -62,7 +62,7 @@ struct RopePlace {
 };
 
 template <typename T, int D, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, 8) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int EPL = ElemTraits<T>::EPL, P = EPL / 2;
   constexpr int LPR = D / EPL;
   extern __shared__ float s_rope[];                  // [2][D] weights, [side * turns_in_row][half] cosine, sine
@@ -254,7 +254,7 @@ extern "C" int ekv_qk_norm_rope(int32_t dtype, int32_t batch, int32_t tokens, in
   // few heads: several tokens side by side.  Many: one token's rows take several turns.
   a.side = all >= slots ? 1 : slots / all;
   a.slots_per_token = slots / a.side;
-  const int64_t want = 4 * sm_count();               // blocks that the GPU holds at a time
+  const int64_t want = 8 * sm_count();               // blocks that the GPU holds at a time
   const int64_t sides = (n_tok + a.side - 1) / a.side;
   // few tokens: the rows of a token are spread over blocks (a decode step is latency); many: a block takes several
   // tokens, whose angles it then computes side by side

@@ -160,19 +160,19 @@ __global__ void __launch_bounds__(256) tree_bounds_kernel(const __grid_constant_
   const int gl = (int)((unsigned)id / (unsigned)a.rows), b = (a.g0 + gl) / a.c.kv_heads;
   const int n = tree_tiles<true>(a, b) * 4;
   const bool live = (a.row0 + (int)id - gl * a.rows) / a.group < tree_drafts(a, b);
+  static_assert(kSampleTiles * 4 == 16 * 32, "a lane holds 16 class maxima");
   tree_wait_for_previous();
   if (!live || n == 0) return;
   const float* const cls = a.classes + id * a.sample_tiles * 4;
-  float t[16];
+  float t[16];                                   // at most kSampleTiles * 4 = 16 * 32 maxima
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    t[i] = -INFINITY;
-    for (int c = i * 32 + lane; c < n; c += 512) t[i] = max_nan(t[i], cls[c]);
-  }
+  for (int i = 0; i < 16; ++i) t[i] = cls[min(i * 32 + lane, n - 1)];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t[i] = i * 32 + lane < n ? t[i] * a.zscale : -INFINITY;
   float top = t[0];
 #pragma unroll
   for (int i = 1; i < 16; ++i) top = max_nan(top, t[i]);
-  top = warp_max_nan(top) * a.zscale;
+  top = warp_max_nan(top);
   const int kind = alpha_kind_of(a.alpha);
   const float beta = 1.f / (a.alpha - 1.f);
   float lo = top - 1.f, hi = top;
@@ -180,8 +180,17 @@ __global__ void __launch_bounds__(256) tree_bounds_kernel(const __grid_constant_
   for (int it = 0; it < 8; ++it) {
     const float mid = 0.5f * (lo + hi);
     float sum = 0.f;
+    if (kind == 1) {                             // alpha 1.5, the usual one, without a branch per score
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += entmax_weight(t[i] * a.zscale, mid, kind, beta);
+      for (int i = 0; i < 16; ++i) {
+        const float d = fmaxf(t[i] - mid, 0.f);
+        sum = fmaf(d, d, sum);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < n; i += 32)
+        if (i + lane < n) sum += entmax_weight(cls[i + lane] * a.zscale, mid, kind, beta);
+    }
     if (warp_sum(sum) >= 1.f) lo = mid; else hi = mid;
   }
   // the roundings of the scaling (2^-24 each) and of the sum: its relative error of 512 2^-24 moves tau by at most
