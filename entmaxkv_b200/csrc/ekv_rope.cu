@@ -11,6 +11,11 @@
 // thread keeps its lane of the row for every head and token that it visits, so the weights of its eight (four) elements
 // stay in registers, the cosines and sines are read once per token, and four rows are on their way while one is worked
 // on.  A block takes several tokens, whose angles it computes first.
+//
+// Measured on a B200: 20,495 tokens of 64 heads of 64, bf16, half rotated: 84 us, 4.0 TB/s, 0.61 of a plain copy (bound by
+// instruction issue: about 85 instructions per 16 bytes, with the products in packed pairs); 512 tokens of 72 heads of
+// 128: 10 us; one token: 4 us.  256-thread blocks took 88 us, cosines and weights held in registers for all heads 137 us
+// (98 registers, two blocks to an SM).
 #include "ekv_common.cuh"
 
 namespace ekv {

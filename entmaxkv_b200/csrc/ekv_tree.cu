@@ -111,6 +111,10 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
 // A warp per row while at most 768 candidates lie above the row's best bound (the usual case: no barrier, sums by
 // shuffle), the whole block per row where more do (flat scores), one such row after another.  Few rows (fewer warps than
 // the GPU holds blocks) get a block each from the start.
+//
+// Bound by latency: the chain lists -> entries -> tau (five or six sums) -> value rows of some 40 keys.  4096 rows of 17k to
+// 32k tokens: 30 us alone, of which most lies behind the last tiles of the score pass; 256 rows with all 4096 scores: 20 us
+// with a block each (38 us with a warp each).
 
 constexpr int kFinWarps = 4;                    // warps of a block that takes a row per warp
 constexpr int kFinOneWarps = 8;                 // and of one that takes a single row
@@ -698,9 +702,12 @@ struct TreePlan {
   TmShape shape;
 };
 
-constexpr int kSampleFrom = 8;         // tiles per block from which on there is a sample (fewer: all scores)
+// Tiles per block from which on there is a sample, and tiles per sequence up to which there need not be one: below both,
+// all scores are written out.  One sequence of 4096 tokens, 32 rows: 35 us without a sample (score pass 15, finish 20); a
+// sample and its bounds alone take 16.  The row of scores that the finish kernel then reads grows with the sequence.
+constexpr int kSampleFrom = 8;
 
-constexpr int kDenseTiles = 64;        // and tiles per sequence up to which that holds
+constexpr int kDenseTiles = 64;
 
 static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
   TreePlan p{};

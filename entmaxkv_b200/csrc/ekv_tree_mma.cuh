@@ -14,6 +14,12 @@
 // tau from below, far closer than the maximum - 1 does.  The bounds do not change during the pass, so the lists do not
 // depend on timing.  Short sequences have no sample: there all scores are written out, which is less than a second launch
 // costs.
+//
+// Measured on a B200 (a launch alone): 8 sequences of 17k to 32k tokens, 64 rows per KV head, 8 heads of 128: sample 20 us,
+// pass 80 us, 387 MB at 4.9 TB/s, 1.2k cycles a tile where it streams; one sequence of 131k tokens, 512 rows per KV head
+// (two blocks of rows share each K tile through L2): pass 155 us, 2.4k cycles a tile of 128 keys by 256 rows, 1.0k of them
+// products; the rest is the epilogue's comparisons and appends.  With keys along the lanes instead of rows the same passes
+// took 112 and 280 us.
 #pragma once
 
 #include <cuda.h>
