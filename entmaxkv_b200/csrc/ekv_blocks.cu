@@ -53,7 +53,9 @@ __device__ __forceinline__ SeqPages seq_pages(const PlanArgs& a, int b) {
     s.more = pages_of(s.seq, a.page_size) - s.held;
   } else {
     s.held = pages_of(s.seq, a.page_size);
-    s.more = pages_of(sat_add(s.seq, s.add), a.page_size) - s.held;
+    // a page behind the table's width takes no block: whoever writes the tokens drops those, too, and the list's top
+    // must stay where the lengths say
+    s.more = max(min(pages_of(sat_add(s.seq, s.add), a.page_size), a.width) - s.held, 0);
   }
   return s;
 }
@@ -106,6 +108,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const __grid_
     held = sat_add(held, s.held);
     tok_end[b] = tokens;
     page_end[b] = pages;
+    if (!RELEASE && a.status && pages_of(sat_add(s.seq, s.add), P) > max(a.width, s.held))
+      atomicOr(a.status, EKV_STATUS_CAPACITY);
   }
   int all_tokens, all_pages, head;
   const int tok_incl = block_scan_sat(tokens, scratch, &all_tokens);

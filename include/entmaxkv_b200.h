@@ -143,7 +143,7 @@ int ekv_extend(const ekv_cache_desc* c, const void* k_new, const void* v_new, in
  * [held[b], need[b]) gets block_table[b, p] = free_blocks[sum(held) + sum_{b' < b}(need - held) + p - held[b]],
  * or -1 past the end of the list.  The list is a stack whose lowest sum(held) places are in use: their
  * content does not matter, and the call changes nothing but table entries behind a sequence's held pages,
- * so it can be repeated.  The new tokens of all sequences, one after another, get
+ * so it can be repeated.  A sequence gets no pages behind the table's width.  The new tokens of all sequences, one after another, get
  *   slots[r] = block * page_size + position % page_size (-1 without a block), positions[r] = position,
  * both -1 from the last token on; row_starts[b] (B + 1 entries) is where sequence b's tokens begin.
  * slots, positions, row_starts and status may be null; status gets EKV_STATUS_CAPACITY when the pool or the

@@ -108,6 +108,36 @@ def test_extend_values_out_of_range_are_clipped_and_reported():
         assert all(0 <= n <= 35 for n in cache.sync_lengths())
 
 
+def test_what_is_not_written_takes_no_block():
+    """Counts beyond the rows given, and pages beyond the table: the pool's top stays where the lengths say, so no block is
+    ever held twice."""
+    import entmaxkv_b200 as E
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    k = rows(3, 1, 8, 64, dtype=torch.float16, seed=40)
+    cache = make_cache(4, "pool", k, k, [4, 4, 8], blocks=30)
+    big = torch.zeros(3, 1, 40, 64, dtype=torch.float16)
+    big[:, :, :8] = k
+    lens = [4, 4, 8]
+    for step, (given, take) in enumerate([([90, 2, 1], [2, 2, 1]), ([2, 70, -5], [2, 2, 0]), ([1, 2, 2], [1, 2, 2]),
+                                          ([2, 2, 2], [2, 2, 2])]):
+        new = rows(3, 1, 2, 64, dtype=torch.float16, seed=41 + step)
+        cache.extend(new.cuda(), new.cuda(), counts=i32(*given))
+        for b in range(3):
+            big[b, :, lens[b]:lens[b] + take[b]] = new[b, :, :take[b]]
+        lens = [n + m for n, m in zip(lens, take)]
+        assert cache.sync_lengths() == lens
+        held = [int(x) for b, n in enumerate(lens) for x in cache._table[b, :-(-n // 4)]]
+        assert len(set(held)) == len(held) and min(held) >= 0
+        for b, n in enumerate(lens):
+            assert torch.equal(cache.k_cache[b, :, :n].cpu(), big[b, :, :n])
+    # a table too narrow for one sequence: the next one's pages follow without a gap
+    table, status = torch.full((2, 2), -1, dtype=torch.int32, device="cuda"), i32(0)
+    slots = torch.zeros(20, dtype=torch.int64, device="cuda")
+    E.plan_block_tables(i32(0, 0), i32(13, 6), table, i32(5, 6, 7, 8, 9), 4, slots=slots, status=status)
+    assert table.tolist() == [[5, 6], [7, 8]] and int(status) == 2
+    assert slots.tolist() == [20, 21, 22, 23, 24, 25, 26, 27, -1, -1, -1, -1, -1, 28, 29, 30, 31, 32, 33, -1]
+
+
 def test_extend_refusals():
     import entmaxkv_b200 as E
     k = rows(2, 2, 32, 64, dtype=torch.float16, seed=8)
