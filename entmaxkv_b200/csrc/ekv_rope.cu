@@ -12,10 +12,10 @@
 // stay in registers, the cosines and sines are read once per token, and four rows are on their way while one is worked
 // on.  A block takes several tokens, whose angles it computes first.
 //
-// Measured on a B200: 20,495 tokens of 64 heads of 64, bf16, half rotated: 84 us, 4.0 TB/s, 0.61 of a plain copy (bound by
+// Measured on a B200: 20,495 tokens of 64 heads of 64, bf16, half rotated: 80 us, 4.2 TB/s, 0.64 of a plain copy (bound by
 // instruction issue: about 85 instructions per 16 bytes, with the products in packed pairs); 512 tokens of 72 heads of
-// 128: 10 us; one token: 4 us.  256-thread blocks took 88 us, cosines and weights held in registers for all heads 137 us
-// (98 registers, two blocks to an SM).
+// 128: 10 us; one token: 4 us.  With a cold cache 84 us, against 88 with 256-thread blocks and 137 with cosines and
+// weights held in registers for all heads (98 registers, two blocks to an SM).
 #include "ekv_common.cuh"
 
 namespace ekv {
