@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
       if (lane < live) {
 #pragma unroll
         for (int j = 0; j < KPW; ++j)
-          if (j < valid && !(acc[j] <= top - 1.f)) list[count++] = make_uint2(__float_as_uint(acc[j]), key0 + warp * KPW + j);
+          // (+inf - +inf is a NaN: an infinite score is listed, though nothing lies above its row's bound)
+          if (j < valid && !(top - acc[j] >= 1.f)) list[count++] = make_uint2(__float_as_uint(acc[j]), key0 + warp * KPW + j);
       }
     }
     if (lane < live) {
@@ -407,7 +408,7 @@ __device__ void fin_block_row(const TreeArgs& a, const FinRow& r, uint2* s_slots
       if (j >= 0 && j < a.tokens) e[k] = make_uint2(__float_as_uint(zd[j]), (uint32_t)~j);     // ~j: drafted
       const float z = __uint_as_float(e[k].x);
       keep[k] = !(z <= floor_z);
-      if (keep[k]) top = max_nan(top, z);
+      top = max_nan(top, z);                     // of all that is read: the floor of an infinite row drops even its maximum
       mine += keep[k];
     }
     int total;
