@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
     if (lane < live) {
       const int64_t at = row_id * a.max_parts * a.sub + part * a.sub + warp;
       a.counts[at] = count;
-      a.bounds[at] = top - 1.f;
+      a.bounds[at] = __fadd_rd(top, -1.f);
     }
   }
 }
@@ -266,46 +266,59 @@ __device__ __forceinline__ void fin_drafts(const TreeArgs& a, const FinRow& r, f
   }
 }
 
-// Root of sum (z - tau)_+^beta = 1 from below.  The norm N(tau) = (sum (z - tau)_+^beta)^(1/beta) falls to 1 at the root and
-// is convex for beta >= 1 (nearly linear when the support is settled), so Newton's steps on it climb towards the root from
-// the left; the bracket keeps them safe for beta < 1.  `sums(tau)` gives sum d^beta and sum d^(beta-1) to every thread.
-template <typename Sums>
-__device__ __forceinline__ float fin_tau(float floor_z, float top, float alpha, int kind, Sums sums) {
-  float lo = floor_z, hi = top, tau = floor_z;
-  for (int it = 0; it < 40; ++it) {
-    const float2 s = sums(tau);
-    if (s.x >= 1.f) lo = tau; else hi = tau;
-    // (N - 1) / -N' = (s0^(1/beta) - 1) s0^(1 - 1/beta) / s1
-    // (the step need not be exact: the sums at the new tau decide)
-    const float root = kind == 0 ? s.x : (kind == 1 ? s.x * rsqrtf(s.x) : pow_pos(s.x, alpha - 1.f));
-    const float step = s.x > 0.f ? __fdividef((root - 1.f) * __fdividef(s.x, root), s.y) : -INFINITY;
-    // half a unit in the last place of the scores that tau is compared with
-    const bool done = fabsf(step) <= 6e-8f * fmaxf(fabsf(tau), fabsf(top));
-    const float next = tau + step;
-    tau = next > lo && next < hi ? next : (done ? tau : 0.5f * (lo + hi));
-    if (done) break;
+// Root of sum (x - tau)_+^beta = 1 from below, x = z - (the row's largest score) and tau = c + t in [-1, 0].  In absolute
+// scores tau would be rounded to a step of the scores' size, and every key of the support takes that error: with alpha 2
+// and 100,000 equal scores of 10 the weights then sum to 0.954.  Relative to the maximum, and in two parts, of which the
+// second holds what the first's step leaves, they sum to one within 1e-6.
+//
+// The norm N(tau) = (sum (x - tau)_+^beta)^(1/beta) falls to 1 at the root and is convex for beta >= 1 (nearly linear when
+// the support is settled), so Newton's steps on it climb towards the root from the left; the bracket keeps them safe.  For
+// beta < 1 (alpha > 2) the sum rises vertically where a key enters, so only the sum itself says when it is enough, and the
+// bracket is halved in its logarithm: n equal scores lie n^-(alpha-1) above the root.  A bracket of two neighbouring numbers
+// moves the origin c there.  Two to eight evaluations as a rule, some 30 for thousands of equal scores near the root, up to
+// 65 for those with alpha above 4.  The sums are taken with d = (x - c) - t.
+struct FinTau {
+  float c, t;            // tau = c + t
+  float lo, hi;          // bracket of t
+};
+constexpr int kFinSteps = 96;
+__device__ __forceinline__ FinTau fin_tau_begin(float floor_x) { return {0.f, floor_x, floor_x, 0.f}; }
+// One step, `s` = sum d^beta, sum d^(beta-1) at f; true: f is the root.
+__device__ __forceinline__ bool fin_tau_step(FinTau& f, float2 s, int it, float alpha, int kind, float beta) {
+  const bool smooth = beta >= 1.f;
+  if (s.x >= 1.f) f.lo = f.t;
+  else f.hi = f.t;
+  if (it == 0 && s.x < 1.f) f.lo = -1.f;
+  // (N - 1) / -N' = (s0^(1/beta) - 1) s0^(1 - 1/beta) / s1
+  // (the step need not be exact: the sums at the new tau decide)
+  const float root = kind == 0 ? s.x : (kind == 1 ? s.x * rsqrtf(s.x) : pow_pos(s.x, alpha - 1.f));
+  const float step = s.x > 0.f ? __fdividef((root - 1.f) * __fdividef(s.x, root), s.y) : -INFINITY;
+  // enough: the sum within the rounding of its terms, or a step of half a unit in the last place
+  bool done = fabsf(s.x - 1.f) <= 5e-7f || (smooth && fabsf(step) <= 6e-8f * fabsf(f.t));
+  if (done && smooth) {
+    const bool first = f.c == 0.f;
+    f.c = first ? f.t : f.c;
+    f.t = first ? step : f.t + step;
   }
-  return tau;
-}
-
-template <int WARPS>
-__device__ __forceinline__ float2 block_sum2(float2 v, float* scratch) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  v.x = warp_sum(v.x);
-  v.y = warp_sum(v.y);
-  __syncthreads();
-  if (lane == 0) {
-    scratch[warp * 2] = v.x;
-    scratch[warp * 2 + 1] = v.y;
+  if (!done) {
+    float next = f.t + step;
+    if (!(next > f.lo && next < f.hi)) {
+      if (smooth || f.hi - f.lo < -0.5f * f.lo) next = 0.5f * (f.lo + f.hi);
+      else next = f.hi < 0.f ? -sqrtf(-f.lo) * sqrtf(-f.hi) : f.lo * 0.015625f;
+    }
+    if (!(next > f.lo && next < f.hi)) {         // two neighbours
+      done = f.c != 0.f || f.hi == 0.f;
+      if (!done) {                               // exact differences from here on: the keys in question lie at c
+        f.c = f.hi;
+        f.lo -= f.hi;
+        f.hi = 0.f;
+        next = f.lo * 0.015625f;
+      }
+    }
+    done |= it == kFinSteps - 1;
+    f.t = done ? f.lo : next;
   }
-  __syncthreads();
-  float2 t = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    t.x += scratch[w * 2];
-    t.y += scratch[w * 2 + 1];
-  }
-  return t;
+  return done;
 }
 
 // exclusive scan of small counts over the block; also the total
@@ -373,7 +386,7 @@ __device__ void fin_block_row(const TreeArgs& a, const FinRow& r, uint2* s_slots
 #pragma unroll 8
     for (int i = tid; i < raw; i += THREADS) top = max_nan(top, z[i]);
     for (int j = tid; j < a.tokens; j += THREADS) top = max_nan(top, zd[j]);
-    floor_z = block_top(top) - 1.f;
+    floor_z = __fadd_rd(block_top(top), -1.f);   // (rounded down: a large maximum must stay above it)
     top = -INFINITY;
   } else {
     const int* const counts = a.counts + r.id * a.max_parts * a.sub;
@@ -427,26 +440,54 @@ __device__ void fin_block_row(const TreeArgs& a, const FinRow& r, uint2* s_slots
     if (tid == 0 && tau_out) *tau_out = top == -INFINITY ? INFINITY : NAN;
     return;
   }
-  const float tau = fin_tau(fmaxf(floor_z, top - 1.f), top, a.alpha, kind, [&](float t) {
-    float2 s = make_float2(0.f, 0.f);
-    float s2 = 0.f;
-    for (int i = tid; i < n; i += THREADS) halley_accumulate(__uint_as_float(rows.get(i).x), t, kind, beta, s.x, s.y, s2);
-    return block_sum2<WARPS>(s, scratch);
-  });
+  // thread 0 makes the steps: all leave the loop by the flag that it writes
+  FinTau tau = fin_tau_begin(fmaxf(floor_z - top, -1.f));
+  __syncthreads();
+  for (int it = 0; it < kFinSteps; ++it) {
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f;
+    for (int i = tid; i < n; i += THREADS)
+      halley_accumulate(__uint_as_float(rows.get(i).x) - top - tau.c, tau.t, kind, beta, s0, s1, s2);
+    s0 = warp_sum(s0);
+    s1 = warp_sum(s1);
+    if (lane == 0) {
+      scratch[warp * 2] = s0;
+      scratch[warp * 2 + 1] = s1;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        s.x += scratch[w * 2];
+        s.y += scratch[w * 2 + 1];
+      }
+      scratch[31] = fin_tau_step(tau, s, it, a.alpha, kind, beta) ? 1.f : 0.f;
+      scratch[30] = tau.t;
+      scratch[29] = tau.c;
+    }
+    __syncthreads();
+    tau.c = scratch[29];
+    tau.t = scratch[30];
+    if (scratch[31] != 0.f) break;
+  }
   int m = 0;
+  float sum_w = 0.f;
   for (int i0 = 0; i0 < n; i0 += THREADS) {
     uint2 e = make_uint2(0, 0);
     float w = 0.f;
     if (i0 + tid < n) {
       e = rows.get(i0 + tid);
-      w = entmax_weight(__uint_as_float(e.x), tau, kind, beta);
+      w = entmax_weight(__uint_as_float(e.x) - top - tau.c, tau.t, kind, beta);
+      sum_w += w;
     }
     int total;
     const int at = m + block_excl<WARPS>(w > 0.f, iscratch, &total);
     if (w > 0.f) rows.put(at, make_uint2(__float_as_uint(w), (uint32_t)fin_pool_key(a, r, (int)e.y)));
     m += total;
   }
-  __syncthreads();
+  // alpha > 2: keys next to the root weigh (rounding)^beta, and no tau that fp32 holds makes thousands of them sum to one
+  sum_w = block_sum(sum_w, scratch);
+  const float scale = beta < 1.f ? 1.f / sum_w : 1.f;
   float acc[EPL] = {};
   const int sub = tid / LPR, col = tid % LPR * EPL;
   for (int i0 = sub; i0 < m; i0 += GROUPS * N) {
@@ -478,9 +519,9 @@ __device__ void fin_block_row(const TreeArgs& a, const FinRow& r, uint2* s_slots
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) s += s_acc[i * D + tid];
-    out[tid] = from_float<T>(s);
+    out[tid] = from_float<T>(s * scale);
   }
-  if (tid == 0 && tau_out) *tau_out = tau;
+  if (tid == 0 && tau_out) *tau_out = top + (tau.c + tau.t);
 }
 
 // A block per row.  Dynamic shared memory: [kFinSlots] slots, [n_lists] lists, [tokens] drafted scores.
@@ -572,7 +613,7 @@ __global__ void __launch_bounds__(kFinWarps * 32, 7) tree_finish_kernel(const __
         most = max_nan(most, __uint_as_float(e[k].x));
       }
       top = max_nan(top, warp_max_nan(most));
-      floor_z = fmaxf(floor_z, top - 1.f);
+      floor_z = fmaxf(floor_z, __fadd_rd(top, -1.f));      // (rounded down: a large maximum must stay above it)
       if (n > kFinLight - 32 * AT_ONCE) {
         int kept = 0;
         for (int j0 = 0; j0 < n; j0 += 32) {
@@ -606,35 +647,35 @@ __global__ void __launch_bounds__(kFinWarps * 32, 7) tree_finish_kernel(const __
       for (int e = lane; e < D; e += 32) out[e] = from_float<T>(top == -INFINITY ? 0.f : NAN);
       if (lane == 0 && tau_out) *tau_out = top == -INFINITY ? INFINITY : NAN;
     } else {
-      const float tau = fin_tau(floor_z, top, a.alpha, kind, [&](float t) {
+      FinTau tau = fin_tau_begin(fmaxf(floor_z - top, -1.f));
+      for (int it = 0; it < kFinSteps; ++it) {
         float2 s = make_float2(0.f, 0.f);
         float s2 = 0.f;
         if (kind == 1) {                         // alpha 1.5, the usual one, without a branch per score
 #pragma unroll 4
           for (int i = lane; i < n; i += 32) {
-            const float d = fmaxf(__uint_as_float(slots[i].x) - t, 0.f);
+            const float d = fmaxf(__uint_as_float(slots[i].x) - top - tau.c - tau.t, 0.f);
             s.x = fmaf(d, d, s.x);
             s.y += d;
           }
         } else {
           for (int i = lane; i < n; i += 32)
-            halley_accumulate(__uint_as_float(slots[i].x), t, kind, beta, s.x, s.y, s2);
+            halley_accumulate(__uint_as_float(slots[i].x) - top - tau.c, tau.t, kind, beta, s.x, s.y, s2);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
-          s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
-        }
-        return s;
-      });
+        s.x = warp_sum(s.x);
+        s.y = warp_sum(s.y);
+        if (fin_tau_step(tau, s, it, a.alpha, kind, beta)) break;      // the same in every lane
+      }
       // the support, in order and in place
       int m = 0;
+      float sum_w = 0.f;
       for (int i0 = 0; i0 < n; i0 += 32) {
         uint2 e = make_uint2(0, 0);
         float w = 0.f;
         if (i0 + lane < n) {
           e = slots[i0 + lane];
-          w = entmax_weight(__uint_as_float(e.x), tau, kind, beta);
+          w = entmax_weight(__uint_as_float(e.x) - top - tau.c, tau.t, kind, beta);
+          sum_w += w;
         }
         const unsigned has = __ballot_sync(0xffffffffu, w > 0.f);
         if (w > 0.f) slots[m + __popc(has & ((1u << lane) - 1))] = make_uint2(__float_as_uint(w), e.y);
@@ -674,10 +715,13 @@ __global__ void __launch_bounds__(kFinWarps * 32, 7) tree_finish_kernel(const __
       for (int o = LPR; o < 32; o <<= 1)
 #pragma unroll
         for (int j = 0; j < EPL; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+      // alpha > 2: keys next to the root weigh (rounding)^beta, and no tau that fp32 holds makes thousands of them sum to one
+      sum_w = warp_sum(sum_w);
+      const float scale = beta < 1.f ? 1.f / sum_w : 1.f;
       if (lane < LPR)
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) out[col + j] = from_float<T>(acc[j]);
-      if (lane == 0 && tau_out) *tau_out = tau;
+        for (int j = 0; j < EPL; ++j) out[col + j] = from_float<T>(acc[j] * scale);
+      if (lane == 0 && tau_out) *tau_out = top + (tau.c + tau.t);
     }
   }
 

@@ -193,7 +193,7 @@ __device__ __forceinline__ void tree_let_next_start() { asm volatile("griddepcon
 
 __device__ __forceinline__ float warp_max_nan(float v) {
   float r;
-  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {      // a NaN stays

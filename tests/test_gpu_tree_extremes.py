@@ -43,3 +43,66 @@ def test_an_infinite_score_makes_its_row_nan_on_every_route(route, where):
     hit[0] = up
     assert out[hit].isnan().all() and tau[hit].isnan().all()
     assert torch.equal(out[~hit], want[~hit]) and torch.equal(tau[~hit], want_tau[~hit])
+
+
+#: rows per KV head and sequences: a block per row, a warp per row
+SHAPES = {"few": (1, 4, 1, 2), "many": (2, 32, 2, 16)}
+PLACES = [(dt, n, shape) for dt in ("bf16", "fp16", "fp32") for n in (40, 4000, 20000) for shape in SHAPES
+          if not (dt == "fp32" and n == 20000 and shape == "many")] + [("bf16", 100000, "few")]
+
+
+def level_scores(dt, n, shape, alpha, score):
+    """Every key and draft scores `score` (exactly: every product and sum is a small multiple of a power of two)."""
+    B, Hq, Hkv, T = SHAPES[shape]
+    x = G.make(B, Hq, Hkv, 64, [1] * B, T, G.DT[dt], seed=52)
+    x["k"] = torch.ones(B, Hkv, n, 64, dtype=G.DT[dt])
+    x["v"] = torch.ones(B, Hkv, n, 64, dtype=G.DT[dt])
+    x["kd"], x["vd"] = torch.ones_like(x["kd"]), torch.ones_like(x["vd"])
+    x["q"] = torch.full_like(x["q"], score / 8 / (alpha - 1))
+    x["mask"] = torch.eye(T, dtype=torch.bool)
+    return x
+
+
+@pytest.mark.parametrize("alpha", [1.5, 2.0, 3.0])
+@pytest.mark.parametrize("dt,n,shape", PLACES)
+def test_weights_of_equal_scores_sum_to_one(dt, n, shape, alpha):
+    """n + 1 equal scores of 8 and values of one: the output is the sum of the weights.  The solver leaves it within
+    1e-6 of one; up to n / 4 additions one after another are off by 2^-24 of the sum each, then one rounding."""
+    x = level_scores(dt, n, shape, alpha, 8.0)
+    out, tau = G.run(x, G.cache_of(x, [n] * SHAPES[shape][0], 16, "dense"), alpha)
+    tol = 1e-6 + (n / 4 + 64) * 2.0 ** -24 + torch.finfo(out.dtype).eps / 2
+    assert (out.double() - 1).abs().max() <= tol
+    # the threshold is rounded to fp32 once: half a step below 8 is 2^-22
+    assert (tau.double() - (8 - (n + 1) ** -(alpha - 1))).abs().max() <= 2.0 ** -22 + 1e-6
+
+
+@pytest.mark.parametrize("alpha", [1.5, 2.0, 2.5, 3.0])
+@pytest.mark.parametrize("dt,n,shape", PLACES)
+def test_many_equal_scores_just_above_the_threshold(dt, n, shape, alpha):
+    """The drafted key scores about 0.875 more than n equal ones, whose weights together have what it leaves of one."""
+    x = level_scores(dt, n, shape, alpha, 8.0)
+    x["kd"] = x["kd"] * 1.109375                # exact in every type: 8 * 1.109375 = 8.875
+    out, _ = G.run(x, G.cache_of(x, [n] * SHAPES[shape][0], 16, "dense"), alpha)
+    tol = 1e-6 + (n / 4 + 64) * 2.0 ** -24 + torch.finfo(out.dtype).eps / 2
+    assert (out.double() - 1).abs().max() <= tol
+
+
+@pytest.mark.parametrize("n", [300, 9000])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_scores_past_what_fp32_counts(dt, shape, n):
+    """Scores of 2^25 and more, where score - 1 is the score again: the largest key has all the weight, two of them half."""
+    B, Hq, Hkv, T = SHAPES[shape]
+    x = G.make(B, Hq, Hkv, 64, [n] * B, T, G.DT[dt], seed=53)
+    x["q"] = torch.zeros_like(x["q"])
+    x["q"][..., 0] = 2.0 ** 15
+    x["k"][..., 0], x["kd"][..., 0] = 2.0 ** 14, 2.0 ** 14
+    x["k"][:, :, 200, 0] = 1.5 * 2.0 ** 14
+    group = Hq // Hkv
+    one, _ = G.run(x, G.cache_of(x, [n] * B, 16, "dense"), 1.5)
+    assert torch.equal(one, x["v"][:, :, 200].repeat_interleave(group, 1)[:, :, None].expand_as(one))
+    x["k"][:, :, 7, 0] = 1.5 * 2.0 ** 14
+    two, _ = G.run(x, G.cache_of(x, [n] * B, 16, "dense"), 1.5)
+    mean = (x["v"][:, :, 200].double() + x["v"][:, :, 7].double()).repeat_interleave(group, 1)[:, :, None] / 2
+    # weights of sqrt(1/2) squared, 2^-22 of each value, and the rounding
+    assert ((two.double() - mean).abs() <= 2.0 ** -21 + (mean.abs() + 2.0 ** -21) * torch.finfo(two.dtype).eps / 2).all()
