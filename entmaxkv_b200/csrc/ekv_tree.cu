@@ -754,9 +754,12 @@ constexpr int kSampleFrom = 8;
 
 constexpr int kDenseTiles = 64;
 
-static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
+// what a launch may use of the GPU's memory before the groups, and where one of them is too large the rows, take turns
+constexpr int64_t kTreeWorkspace = (int64_t)6 << 30;
+
+static TreePlan tree_plan_rows(const ekv_cache_desc* c, int rows, int tokens, int max_seq) {
   TreePlan p{};
-  p.rows = tokens * (q_heads / c->kv_heads);
+  p.rows = rows;
   p.mma = c->dtype != EKV_F32;
   p.tile_keys = kTreeTile;
   p.list_turn = 1;
@@ -797,6 +800,18 @@ static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int 
   return p;
 }
 
+// The plan of a turn: all rows of a group, or as many as the workspace holds (whole blocks of rows where it can be).
+static TreePlan tree_plan(const ekv_cache_desc* c, int q_heads, int tokens, int max_seq) {
+  int64_t rows = (int64_t)tokens * (q_heads / c->kv_heads);
+  for (;;) {
+    const TreePlan p = tree_plan_rows(c, (int)rows, tokens, max_seq);
+    if (p.row_bytes * rows <= kTreeWorkspace || rows == 1) return p;
+    rows = kTreeWorkspace / p.row_bytes;           // fewer; with fewer rows a row may have more pieces, hence more bytes
+    if (rows >= kTmMaxRows) rows = rows / kTmMaxRows * kTmMaxRows;
+    if (rows < 1) rows = 1;
+  }
+}
+
 // K as the copies see it: [blocks or sequences][KV heads][rows][D]
 static int tree_k_map(CUtensorMap* map, const ekv_cache_desc* c, int box_rows) {
   static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
@@ -823,9 +838,6 @@ static int tree_k_map(CUtensorMap* map, const ekv_cache_desc* c, int box_rows) {
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? EKV_OK : EKV_ERR_ARG;
 }
-
-// what a launch may use of the GPU's memory before the groups are taken in several turns
-constexpr int64_t kTreeWorkspace = (int64_t)6 << 30;
 
 static int64_t tree_groups_per_turn(const TreePlan& p, int groups) {
   int64_t n = kTreeWorkspace / (p.row_bytes * p.rows);
@@ -862,7 +874,7 @@ static int launch_scores(const TreeArgs& a, const TreePlan& p, const CUtensorMap
     };
     if (p.dense) return run(tree_scores_mma_kernel<T, D, TM_DENSE>, false);
     if (int e = run(tree_scores_mma_kernel<T, D, TM_SAMPLE>, false)) return e;
-    const int64_t rows = (int64_t)(a.g1 - a.g0) * p.rows;
+    const int64_t rows = (int64_t)(a.g1 - a.g0) * a.rows;
     const cudaError_t e = launch_after(tree_bounds_kernel, (unsigned)((rows + 7) / 8), 256, 0, st, true, a, rows);
     if (e != cudaSuccess) return (int)e;
     return run(tree_scores_mma_kernel<T, D, TM_LISTS>, true);
@@ -940,8 +952,6 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   a.alpha = alpha;
   a.zscale = (float)(((double)alpha - 1.0) / sqrt((double)c->head_dim));
   a.max_seq = max_seq_len;
-  a.row0 = 0;
-  a.rows = p.rows;
   a.ranges = p.ranges;
   a.row_blocks = p.row_blocks;
   a.sub = p.sub;
@@ -966,24 +976,28 @@ extern "C" int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int
   CUtensorMap k_map{};
   if (p.mma && max_seq_len > 0)
     if (int e = tree_k_map(&k_map, c, p.shape.box_rows)) return e;
-  for (int g0 = 0; g0 < groups; g0 += (int)turn) {
-    a.g0 = g0;
-    a.g1 = (int)(g0 + turn < groups ? g0 + turn : groups);
-    const int64_t rows = (int64_t)(a.g1 - g0) * p.rows;
-    if (rows > 0x7fffffff) return EKV_ERR_ARG;
-    int err = EKV_OK;
-    EKV_DISPATCH(c->dtype, c->head_dim, {
-      if (max_seq_len > 0) err = launch_scores<T, D>(a, p, k_map, st);
-      if (err) return err;
-      const auto finish = [&](auto kernel, unsigned grid, int threads, auto... args) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fin_smem);
-        return e != cudaSuccess ? e : launch_after(kernel, grid, threads, fin_smem, st, max_seq_len > 0, a, args...);
-      };
-      const cudaError_t e = one ? finish(tree_finish_one_kernel<T, D>, (unsigned)rows, kFinOneWarps * 32, n_lists)
-                                : finish(tree_finish_kernel<T, D>, (unsigned)((rows + kFinWarps - 1) / kFinWarps),
-                                         kFinWarps * 32, rows, n_lists);
-      if (e != cudaSuccess) return (int)e;
-    });
-  }
+  const int all_rows = tokens * a.group;
+  for (int g0 = 0; g0 < groups; g0 += (int)turn)
+    for (int row0 = 0; row0 < all_rows; row0 += p.rows) {
+      a.g0 = g0;
+      a.g1 = (int)(g0 + turn < groups ? g0 + turn : groups);
+      a.row0 = row0;
+      a.rows = p.rows < all_rows - row0 ? p.rows : all_rows - row0;
+      const int64_t rows = (int64_t)(a.g1 - g0) * a.rows;
+      if (rows > 0x7fffffff) return EKV_ERR_ARG;
+      int err = EKV_OK;
+      EKV_DISPATCH(c->dtype, c->head_dim, {
+        if (max_seq_len > 0) err = launch_scores<T, D>(a, p, k_map, st);
+        if (err) return err;
+        const auto finish = [&](auto kernel, unsigned grid, int threads, auto... args) {
+          const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fin_smem);
+          return e != cudaSuccess ? e : launch_after(kernel, grid, threads, fin_smem, st, max_seq_len > 0, a, args...);
+        };
+        const cudaError_t e = one ? finish(tree_finish_one_kernel<T, D>, (unsigned)rows, kFinOneWarps * 32, n_lists)
+                                  : finish(tree_finish_kernel<T, D>, (unsigned)((rows + kFinWarps - 1) / kFinWarps),
+                                           kFinWarps * 32, rows, n_lists);
+        if (e != cudaSuccess) return (int)e;
+      });
+    }
   return launch_status();
 }

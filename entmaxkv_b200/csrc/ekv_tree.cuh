@@ -9,7 +9,8 @@
 //            classes of keys; a small kernel makes their tau the row's bound.
 //   scores   one pass over K.  The rows that share a KV head are scored together, and each row keeps a list of the
 //            (z, key) above its bound.
-//   finish   one block per row: adds the drafted keys, solves tau on the lists and sums the value rows of the support.
+//   finish   a warp per row, or a block where rows are few or a row's list is long: adds the drafted keys, solves tau on the
+//            lists and sums the value rows of the support.
 //            V is read only where a weight is non-zero.
 //
 // Work split of a pass over K: its 128-key tiles of all (sequence, KV head) groups in a row, cut into `ranges` equal

@@ -35,7 +35,8 @@ def tree_attention_decode(q: torch.Tensor, kv_cache: PagedKVCache, k_draft: torc
     no longer moves; ``out = sum p v``, written in place and returned.  A row that sees nothing gets zeros and
     ``tau = +inf``; a NaN or +inf score makes its row NaN (output and threshold), a score of -inf is as if unseen.  ``taus_out`` (fp32 [B, H_q, T], contiguous) receives the
     thresholds.  Works on dense and block-table caches; the cache is not changed.  ``out`` must not overlap the inputs.
-    Scratch comes from torch's allocator, about 8 bytes per row and cached token up to 6 GiB, of which little is touched.
+    Scratch comes from torch's allocator in each call: about 8 bytes per row and cached token (of the capacity, where the
+    call is captured or captured calls add tokens), at most 6 GiB: then groups of rows take turns.  Little of it is touched.
     """
     if kv_cache._k is None:
         raise RuntimeError("kv_cache is not initialised")

@@ -327,7 +327,7 @@ int ekv_tau_clamp(const float* tau_hat, int64_t tau_hat_stride, const float* cap
  * they were.  The cache is only read.  Strides {batch, head, token} in elements; tau [B, H_q, tokens]
  * contiguous, may be null.  max_seq_len: host-side upper bound of seq_lens[], at most the capacity (longer
  * sequences are cut to it).  The workspace needs no initialisation; its size grows with rows * max_seq_len
- * up to about 6 GiB, then the (sequence, KV head) groups are taken in several turns.
+ * up to 6 GiB, then the (sequence, KV head) groups, and the rows of a group that needs more, take turns.
  * The reference decodes one token at a time (entmaxkv/attention_topk.py:8-100). */
 size_t ekv_tree_workspace_bytes(const ekv_cache_desc* c, int32_t q_heads, int32_t tokens, int32_t max_seq_len);
 int ekv_tree_decode(const ekv_cache_desc* c, const void* q, const int64_t* q_strides, int32_t q_heads,

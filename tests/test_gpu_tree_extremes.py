@@ -106,3 +106,33 @@ def test_scores_past_what_fp32_counts(dt, shape, n):
     mean = (x["v"][:, :, 200].double() + x["v"][:, :, 7].double()).repeat_interleave(group, 1)[:, :, None] / 2
     # weights of sqrt(1/2) squared, 2^-22 of each value, and the rounding
     assert ((two.double() - mean).abs() <= 2.0 ** -21 + (mean.abs() + 2.0 ** -21) * torch.finfo(two.dtype).eps / 2).all()
+
+
+def test_rows_of_one_group_take_turns():
+    """2048 rows of one KV head over 524,288 tokens: their scratch would be 8.6 GB, so the rows take turns.  The same as
+    half of the query heads at a time, which fit; a tree that ends inside the second turn leaves the rest as it was."""
+    import entmaxkv_b200 as E
+    S, T, Hq, D = 524288, 256, 8, 64
+    g = torch.Generator(device="cuda").manual_seed(54)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    q, kd, vd = r(1, Hq, T, D), r(1, 1, T, D), r(1, 1, T, D)
+    cache = E.PagedKVCache(16, capacity=S)
+    cache.initialize(r(1, 1, S, D), r(1, 1, S, D))
+    mask = torch.ones(T, T, dtype=torch.bool, device="cuda").tril()
+    live = torch.tensor([201], dtype=torch.int32, device="cuda")
+    outs = []
+    for heads in (slice(0, 8), slice(0, 4), slice(4, 8)):
+        out, tau = torch.full_like(q[:, heads], 7.0), torch.full(q[:, heads].shape[:3], 7.0, device="cuda")
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        E.tree_attention_decode(q[:, heads], cache, kd, vd, mask, out, draft_lens=live, taus_out=tau)
+        assert torch.cuda.max_memory_allocated() - before <= (6 << 30) + (1 << 20)
+        outs.append((out, tau))
+    torch.cuda.synchronize()
+    assert cache.device_status() == 0
+    whole, half = outs[0], [torch.cat(x, dim=1) for x in zip(*outs[1:])]
+    assert (whole[0][:, :, 201:] == 7).all() and (whole[1][:, :, 201:] == 7).all()
+    # the pieces of the tile sequence differ, and with them the order of the sums: one bf16 step, and rarely that
+    assert (whole[0].float() - half[0].float()).abs().max() <= 2 * 2.0 ** -8 * half[0][:, :, :201].float().abs().max()
+    assert (whole[0] == half[0]).float().mean() > 0.99
+    assert (whole[1] - half[1]).abs().max() <= 1e-5

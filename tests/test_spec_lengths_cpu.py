@@ -1,0 +1,26 @@
+"""Host side of the speculative step, without a GPU: sizes of the scratch, and lengths that the host only bounds."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from tests.test_spec_cpu import desc, fake, lib  # noqa: F401  (lib: a fixture)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("table", [False, True])
+@pytest.mark.parametrize("q_heads,tokens,most", [(8, 256, 1 << 20), (64, 256, 131072), (32, 200, 100003), (512, 256, 1 << 16),
+                                                 (1, 1, 1 << 24), (16, 256, (1 << 22) + 5)])
+def test_scratch_of_one_group_is_bounded(lib, dtype, table, q_heads, tokens, most):  # noqa: F811
+    """More rows of a single KV head than 6 GiB hold at 8 bytes per row and token: they take turns."""
+    buf, p = fake()
+    cap = (most + 15) // 16 * 16
+    d = desc(p, batch=1, kv_heads=1, capacity=cap, page_capacity=cap // 16, kv_stride_h=64 * cap, kv_stride_b=64 * cap,
+             dtype=dtype)
+    if table:
+        d.block_table, d.bt_stride, d.kv_stride_block, d.num_blocks = p, cap // 16, 64 * 16, cap // 16
+    size = lib.ekv_tree_workspace_bytes(C.byref(d), q_heads, tokens, most)
+    assert 0 < size <= (6 << 30) + 256
+    if q_heads * tokens * most * 8 < 5 << 30:
+        assert size >= q_heads * tokens * most * 4          # what fits is not cut: a score takes four bytes at least
