@@ -111,14 +111,21 @@ class DecodeStepGraph:
 
     def _capture(self, with_io: bool = False):
         cache = self.cache
-        # one eager pass without the append allocates every scratch buffer outside the capture
+        # one eager pass without the append allocates every scratch buffer outside the capture.  Where a sequence may
+        # hold no token yet, the pass appends this step's, and the lengths are put back: the replay writes the same again
+        lens, empty = list(cache._host_lens), cache._may_be_empty
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
-            self._call(append=False)
+            device_lens = cache.seq_lens.clone() if empty else None
+            try:
+                self._call(append=empty)
+            finally:
+                if empty:
+                    cache.seq_lens.copy_(device_lens)
+                    cache._host_lens, cache._may_be_empty = list(lens), True
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
-        lens = list(cache._host_lens)
         g = torch.cuda.CUDAGraph()
         # a step that holds a collective (``sigma_mean`` given as a callable) is captured in
         # thread-local mode: the process group's watchdog thread keeps polling while this one captures
@@ -160,10 +167,10 @@ class DecodeStepGraph:
         io = self.pinned_io()
         cache._make_room([n + 1 for n in cache._host_lens])
         if self.graph_io is None or self._captured_capacity_io != cache.capacity:
-            self.q.copy_(io["q"], non_blocking=True)      # the capture's eager warm-up pass runs on the real query
+            self._in.copy_(self._pinned_in, non_blocking=True)      # the capture's eager warm-up pass runs on the real step
             self._capture(with_io=True)
         self.graph_io.replay()
-        cache._host_lens = [n + 1 for n in cache._host_lens]
+        self._appended()
         return io["out"]
 
     def step(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> torch.Tensor:
@@ -175,5 +182,10 @@ class DecodeStepGraph:
         if self.graph is None or self._captured_capacity != cache.capacity:
             self._capture()
         self.graph.replay()
-        cache._host_lens = [n + 1 for n in cache._host_lens]
+        self._appended()
         return self.out
+
+    def _appended(self):
+        """A replay gave every sequence a token."""
+        self.cache._host_lens = [n + 1 for n in self.cache._host_lens]
+        self.cache._may_be_empty = False

@@ -1,0 +1,70 @@
+"""Lengths of the cache that shrink, grow unseen by the host, or are only bounded there (run on a B200: ``-m gpu``)."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(*shape, seed):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).bfloat16().cuda()
+
+
+def make(layout, lens, page=16, blocks=200, capacity=None):
+    import entmaxkv_b200 as E
+    kw = dict(block_table=True, num_blocks=blocks) if layout == "pool" else {}
+    c = E.PagedKVCache(page, capacity=capacity, **kw)
+    k, v = rows(len(lens), 2, max(lens), 128, seed=1), rows(len(lens), 2, max(lens), 128, seed=2)
+    c.initialize(k, v, seq_lens=lens)
+    return c
+
+
+def eager(cache, mode, q, k, v):
+    import entmaxkv_b200 as E
+    out = torch.zeros_like(q)
+    if mode == "topk":
+        E.sparse_attention_decode_paged(q, cache, k, v, out, 64, alpha=1.5, niter=10)
+    else:
+        E.sparse_attention_decode_gaussian_aware_entmax(q, cache, k, v, out, alpha=1.5, append_cache=True)
+    return out
+
+
+@pytest.mark.parametrize("layout", ["dense", "pool"])
+@pytest.mark.parametrize("mode", ["topk", "gaussian"])
+@pytest.mark.parametrize("pinned", [False, True])
+def test_captured_steps_after_a_release(layout, mode, pinned):
+    """A released sequence starts again through captured steps: the first capture, replays, and the capture that follows
+    when the cache has to grow give what eager steps give."""
+    from entmaxkv_b200.graph import DecodeStepGraph
+    lens = [70, 90]
+    one, two = make(layout, lens, capacity=96), make(layout, lens, capacity=96)
+    kw = dict(token_budget=64) if mode == "topk" else {}
+    graph = DecodeStepGraph(one, 4, mode, alpha=1.5, niter=10 if mode == "topk" else 2, **kw)
+    for c in (one, two):
+        c.release([0])
+    for step in range(40):
+        if step == 25:
+            for c in (one, two):
+                c.release([1])
+        q, k, v = (rows(2, n, 1, 128, seed=10 * step + n) for n in (4, 2, 2))
+        k, v = k, v * 0.5
+        if pinned:
+            io = graph.pinned_io()
+            for name, t in (("q", q), ("k_new", k), ("v_new", v)):
+                io[name].copy_(t)
+            graph.step_pinned()
+            torch.cuda.synchronize()
+            got = io["out"].cuda()
+        else:
+            got = graph.step(q, k, v).clone()
+        want = eager(two, mode, q, k, v)
+        # the wider table of a grown cache may take another kernel: equal up to two roundings to bf16
+        assert (got.float() - want.float()).abs().max() <= 2 * 2.0 ** -8 * max(want.abs().max().item(), 1e-3), step
+        assert one.host_seq_lens == two.host_seq_lens and torch.equal(one.seq_lens, two.seq_lens), step
+    assert one.seq_lens.tolist() == [40, 15] and one.device_status() == 0
+    for b, n in enumerate(one.host_seq_lens):
+        for name in ("k_cache", "v_cache"):
+            assert torch.equal(getattr(one, name)[b, :, :n], getattr(two, name)[b, :, :n])
+    # every sequence holds tokens again: an eager step without an append is not refused
+    import entmaxkv_b200 as E
+    E.sparse_attention_decode_paged(q, one, None, None, torch.zeros_like(q), 64, append_cache=False)
