@@ -305,14 +305,15 @@ class PagedKVCache:
             self.extend(k_new, v_new)
             return
         self._make_room([n + 1 for n in self._host_lens])
-        self._grows_in_graphs |= torch.cuda.is_current_stream_capturing()
+        capturing = torch.cuda.is_current_stream_capturing()
+        self._grows_in_graphs |= capturing
         lib = _lib.load()
         _lib.check(lib.ekv_append(C.byref(self.desc()), k_new.data_ptr(), v_new.data_ptr(),
                                   k_new.stride(0), k_new.stride(1),
                                   self._ctl[16:].data_ptr(), self._ctl.data_ptr(), _lib.stream_ptr()),
                    "ekv_append")
         self._host_lens = [n + 1 for n in self._host_lens]
-        self._may_be_empty = False
+        self._may_be_empty &= capturing        # a capture appends nothing yet
 
     def extend(self, k_new: torch.Tensor, v_new: torch.Tensor, counts=None, index: Optional[torch.Tensor] = None,
                start=None, max_seq_len: Optional[int] = None):
@@ -364,7 +365,8 @@ class PagedKVCache:
             s = k_new.stride()
         with _lib.on_device(dev):
             self._make_room(bound)
-            self._grows_in_graphs |= torch.cuda.is_current_stream_capturing()
+            capturing = torch.cuda.is_current_stream_capturing()
+            self._grows_in_graphs |= capturing
             if self.num_blocks is not None:
                 held = self.seq_lens
                 if start is not None:          # what lies behind the rewind goes back first
@@ -382,7 +384,7 @@ class PagedKVCache:
         if counts_host is None or rewound_on_device:
             self._lens_exact = False
         if counts_host is not None and min(counts_host) > 0:
-            self._may_be_empty = False
+            self._may_be_empty &= capturing    # a capture writes nothing yet
         elif rewound_on_device or (start_host is not None and 0 in start_host):
             self._may_be_empty = True
         self._host_lens = bound

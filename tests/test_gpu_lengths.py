@@ -68,3 +68,21 @@ def test_captured_steps_after_a_release(layout, mode, pinned):
     # every sequence holds tokens again: an eager step without an append is not refused
     import entmaxkv_b200 as E
     E.sparse_attention_decode_paged(q, one, None, None, torch.zeros_like(q), 64, append_cache=False)
+
+
+def test_a_capture_alone_gives_no_sequence_a_token():
+    import entmaxkv_b200 as E
+    cache = make("dense", [40, 40])
+    k = rows(2, 2, 1, 128, seed=3)
+    cache.release([1])
+    for call in (lambda: cache.append(k, k), lambda: cache.extend(k, k)):
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            call()
+        q = rows(2, 4, 1, 128, seed=4)
+        with pytest.raises(ValueError):
+            E.sparse_attention_decode_paged(q, cache, None, None, torch.zeros_like(q), 64, append_cache=False)
+    graph.replay()
+    assert cache.sync_lengths() == [41, 1]
+    E.sparse_attention_decode_paged(q, cache, None, None, torch.zeros_like(q), 64, append_cache=False)
