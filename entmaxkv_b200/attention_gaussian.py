@@ -207,8 +207,8 @@ def sparse_attention_decode_gaussian_aware_entmax(
     _check_q_out(q, out, kv_cache)
     if append_cache:
         kv_cache.append(k_new, v_new)
-    elif kv_cache._may_be_empty:
-        raise ValueError("a sequence may hold no token: give it some, or call kv_cache.sync_lengths()")
+    else:
+        kv_cache.require_tokens()
     B, Hq, _, D = q.shape
     frac = 0.1 if threshold_excess_margin_fraction is None else threshold_excess_margin_fraction
     alibi = None

@@ -268,8 +268,8 @@ def sparse_attention_decode_paged(
     _check_q_out(q, out, kv_cache)
     if append_cache:
         kv_cache.append(k_new, v_new)
-    elif kv_cache._may_be_empty:
-        raise ValueError("a sequence may hold no token: give it some, or call kv_cache.sync_lengths()")
+    else:
+        kv_cache.require_tokens()
     B, Hq, _, D = q.shape
     P = kv_cache.page_size
     alibi = None if alibi_slopes is None else _alibi_args(alibi_slopes, q_seqlens, B, Hq, q.device)

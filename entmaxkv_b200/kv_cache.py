@@ -443,6 +443,11 @@ class PagedKVCache:
         self._host_lens = [0 if i in rows else n for i, n in enumerate(self._host_lens)]
         self._may_be_empty = True
 
+    def require_tokens(self):
+        """What attends to a cache, or selects pages of it, is defined for sequences of at least one token."""
+        if self._may_be_empty:
+            raise ValueError("a sequence may hold no token: give it some, or call kv_cache.sync_lengths()")
+
     # ------------------------------------------------------------------ C ABI view
 
     def desc(self) -> _lib.CacheDesc:
@@ -500,6 +505,7 @@ class PagedKVCache:
         """
         if not exclude_last_page:
             raise NotImplementedError("only exclude_last_page=True is implemented")
+        self.require_tokens()
         from .attention_topk import _alibi_args, _score_and_select
         alibi = None
         if alibi_slopes is not None:
@@ -526,6 +532,7 @@ class PagedKVCache:
         call stay in ``last_gaussian_selection``.
         """
         from .attention_gaussian import gaussian_select
+        self.require_tokens()
         stats = gaussian_stats or {}
         frac = stats.get("threshold_excess_margin_fraction", 0.1)
         frac = 0.1 if frac is None else frac

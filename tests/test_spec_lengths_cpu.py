@@ -24,3 +24,23 @@ def test_scratch_of_one_group_is_bounded(lib, dtype, table, q_heads, tokens, mos
     assert 0 < size <= (6 << 30) + 256
     if q_heads * tokens * most * 8 < 5 << 30:
         assert size >= q_heads * tokens * most * 4          # what fits is not cut: a score takes four bytes at least
+
+
+def host_cache(lens, capacity=64, page=16, **kw):
+    """A cache whose buffers lie on the CPU: what the host decides before a launch can be tried without a GPU."""
+    import entmaxkv_b200 as E
+    c = E.PagedKVCache(page, **kw)
+    c._allocate(len(lens), 2, 64, capacity, torch.bfloat16, "cpu")
+    c._host_lens, c.seq_lens = list(lens), torch.tensor(lens, dtype=torch.int32)
+    c._ctl = torch.zeros(16 + len(lens), dtype=torch.int32)
+    return c
+
+
+def test_selection_helpers_refuse_sequences_without_tokens():
+    cache = host_cache([20, 0])
+    cache._may_be_empty = True
+    q = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="no token"):
+        cache.estimate_page_criticality(q, exclude_last_page=True)
+    with pytest.raises(ValueError, match="no token"):
+        cache.select_gaussian_aware(q)
