@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from .attention_gaussian import sparse_attention_decode_gaussian_aware_entmax
 from .attention_topk import sparse_attention_decode_paged
-from .kv_cache import PagedKVCache
+from .kv_cache import PagedKVCache, _one_more
 
 
 def stage_inputs(pairs) -> None:
@@ -165,7 +165,7 @@ class DecodeStepGraph:
         valid once the current stream has been synchronised."""
         cache = self.cache
         io = self.pinned_io()
-        cache._make_room([n + 1 for n in cache._host_lens])
+        cache._room_for(_one_more)
         if self.graph_io is None or self._captured_capacity_io != cache.capacity:
             self._in.copy_(self._pinned_in, non_blocking=True)      # the capture's eager warm-up pass runs on the real step
             self._capture(with_io=True)
@@ -175,7 +175,7 @@ class DecodeStepGraph:
 
     def step(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> torch.Tensor:
         cache = self.cache
-        cache._make_room([n + 1 for n in cache._host_lens])
+        cache._room_for(_one_more)
         # inputs first: the eager warm-up pass of a (re)capture then runs on this step's real query
         # (an all-zero query would make every page pass the Gaussian threshold)
         stage_inputs(((self.q, q), (self.k_new, k_new), (self.v_new, v_new)))
@@ -187,5 +187,5 @@ class DecodeStepGraph:
 
     def _appended(self):
         """A replay gave every sequence a token."""
-        self.cache._host_lens = [n + 1 for n in self.cache._host_lens]
+        self.cache._host_lens = _one_more(self.cache._host_lens)
         self.cache._may_be_empty = False

@@ -33,6 +33,10 @@ import torch
 from . import _lib
 
 
+def _one_more(lens):
+    return [n + 1 for n in lens]
+
+
 class PagedKVCache:
     """KV cache with min/max/mean/std statistics per page of ``page_size`` keys."""
 
@@ -304,7 +308,7 @@ class PagedKVCache:
         if self.num_blocks is not None:        # a new page needs its block first
             self.extend(k_new, v_new)
             return
-        self._make_room([n + 1 for n in self._host_lens])
+        lens = self._room_for(_one_more)
         capturing = torch.cuda.is_current_stream_capturing()
         self._grows_in_graphs |= capturing
         lib = _lib.load()
@@ -312,7 +316,7 @@ class PagedKVCache:
                                   k_new.stride(0), k_new.stride(1),
                                   self._ctl[16:].data_ptr(), self._ctl.data_ptr(), _lib.stream_ptr()),
                    "ekv_append")
-        self._host_lens = [n + 1 for n in self._host_lens]
+        self._host_lens = lens
         self._may_be_empty &= capturing        # a capture appends nothing yet
 
     def extend(self, k_new: torch.Tensor, v_new: torch.Tensor, counts=None, index: Optional[torch.Tensor] = None,
@@ -328,7 +332,10 @@ class PagedKVCache:
         its view of the lengths (``seq_len``, ``host_seq_lens``, the row range of ``k_cache``) becomes an upper bound:
         ``T`` more tokens for every sequence, or ``max_seq_len`` where that is given and smaller (rows past it are then
         the caller's mistake).  ``sync_lengths`` makes it exact again; call it after replays of a captured ``extend``, too,
-        which the host does not count.  Values out of range are clipped on the device and show in ``device_status``.
+        which the host does not count.  Scratch and work of later calls are sized by the bound, so a loop does well to
+        pass ``max_seq_len`` or to call ``sync_lengths`` now and then.  Where the bound leaves no room in the buffers or in
+        the pool, the call reads the lengths itself (one synchronisation) before it grows the cache or gives up.
+        Values out of range are clipped on the device and show in ``device_status``.
         ``k_new`` and ``v_new`` must not be views of the cache itself.
         """
         if self._k is None:
@@ -348,23 +355,27 @@ class PagedKVCache:
             raise ValueError(f"index must be int32 [{B}, {T}], contiguous along the tokens")
         counts_host, counts = self._row_lens(counts, "counts", T)
         start_host, start = self._row_lens(start, "start", None)
-        bound = self._host_lens if start_host is None else [min(s, n) for s, n in zip(start_host, self._host_lens)]
-        bound = [n + T for n in bound] if counts_host is None else [n + m for n, m in zip(bound, counts_host)]
-        if max_seq_len is not None and max(bound) > max_seq_len:
-            bound = [n if n < max_seq_len else max_seq_len for n in bound]
+
+        def after(lens):
+            lens = lens if start_host is None else [min(s, n) for s, n in zip(start_host, lens)]
+            lens = [n + T for n in lens] if counts_host is None else [n + m for n, m in zip(lens, counts_host)]
+            if max_seq_len is not None and max(lens) > max_seq_len:
+                lens = [n if n < max_seq_len else max_seq_len for n in lens]
+            return lens
+
         rewound_on_device = start is not None and start_host is None
         if T == 0:
             if start is None:
                 return
             k_new = v_new = k_new.new_zeros(B, H, 1, D)      # a rewind alone: no row is taken
-            counts, T, index = torch.zeros(B, dtype=torch.int32, device=device), 1, None
+            counts, counts_host, T, index = torch.zeros(B, dtype=torch.int32, device=device), [0] * B, 1, None
         e = k_new.element_size()
         s = k_new.stride()
         if s != v_new.stride() or s[3] != 1 or (s[0] | s[1] | s[2]) * e % 16 or (k_new.data_ptr() | v_new.data_ptr()) % 16:
             k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
             s = k_new.stride()
         with _lib.on_device(dev):
-            self._make_room(bound)
+            bound = self._room_for(after)
             capturing = torch.cuda.is_current_stream_capturing()
             self._grows_in_graphs |= capturing
             if self.num_blocks is not None:
@@ -389,14 +400,28 @@ class PagedKVCache:
             self._may_be_empty = True
         self._host_lens = bound
 
+    def _room_for(self, after):
+        """Room for the tokens of a call: ``after`` gives its lengths from those before it.  Returns them, with
+        ``_host_lens`` brought up to date where it only bounded the lengths and the bound, not the tokens, leaves no room."""
+        lens = after(self._host_lens)
+        if max(lens) > self.capacity or not self._pool_suffices(lens):
+            if (self._grows_in_graphs or not self._lens_exact) and not torch.cuda.is_current_stream_capturing():
+                self.sync_lengths()
+                lens = after(self._host_lens)
+            self._make_room(lens)
+        return lens
+
+    def _pool_suffices(self, lens):
+        return self.num_blocks is None or sum(-(-n // self.page_size) for n in lens) <= self.num_blocks
+
     def _make_room(self, lens):
         """Before tokens are added: room for sequences of ``lens`` tokens (upper bounds), and blocks in a shared pool."""
+        if not self._pool_suffices(lens):
+            raise RuntimeError(f"the pool of {self.num_blocks} blocks may not suffice: release() sequences" + (
+                "" if self._lens_exact else ", or call sync_lengths() (the host knows only upper bounds of the lengths)"))
         most = max(lens)
         if most > self.capacity:
             self.reserve(max(most, self.capacity + 4096, self.capacity * 5 // 4))
-        if self.num_blocks is not None and sum(-(-n // self.page_size) for n in lens) > self.num_blocks:
-            raise RuntimeError(f"the pool of {self.num_blocks} blocks may not suffice: release() sequences" + (
-                "" if self._lens_exact else ", or call sync_lengths() (the host knows only upper bounds of the lengths)"))
 
     def _row_lens(self, value, name, most):
         """One length per sequence, given on the host or on the device: (host list or None, int32 CUDA tensor or None)."""

@@ -26,6 +26,9 @@ def tree_attention_decode(q: torch.Tensor, kv_cache: PagedKVCache, k_draft: torc
                           alpha: float = 1.5, taus_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attend with T drafted tokens per sequence to the whole cache and to each token's part of the tree.
 
+    All pages, without ALiBi: a one-token step that selects pages attends to less, and equals this one when its budget
+    covers the cache.
+
     q, out [B, H_q, T, D]; k_draft, v_draft [B, H_kv, T, D] in the cache's dtype (any strides).  ``tree_mask``: bool,
     [T, T] or [B, T, T]: token t sees drafted token j where ``tree_mask[..., t, j]`` (itself included only where it says
     so), and every token of the cache.  ``draft_lens`` (int32 CUDA [B]): trees of different sizes; tokens from there on

@@ -86,3 +86,21 @@ def test_a_capture_alone_gives_no_sequence_a_token():
     graph.replay()
     assert cache.sync_lengths() == [41, 1]
     E.sparse_attention_decode_paged(q, cache, None, None, torch.zeros_like(q), 64, append_cache=False)
+
+
+@pytest.mark.parametrize("layout", ["dense", "pool"])
+def test_the_loop_runs_as_long_as_its_tokens_fit(layout):
+    """Eight drafts a step of which one or two are accepted, counts on the device only: 60 steps would bound the lengths by
+    500, the tokens fit in 160."""
+    cache = make(layout, [40, 33], blocks=20, capacity=160)
+    lens = [40, 33]
+    buffers = cache._meta.data_ptr()
+    for step in range(60):
+        k = rows(2, 2, 8, 128, seed=step)
+        take = [1 + step % 2, 1]
+        cache.extend(k, k, counts=torch.tensor(take, dtype=torch.int32, device="cuda"))
+        lens = [n + m for n, m in zip(lens, take)]
+        assert all(h >= n for h, n in zip(cache.host_seq_lens, lens))
+        assert torch.equal(cache.k_cache[0, :, lens[0] - 1], k[0, :, take[0] - 1])
+    assert cache._meta.data_ptr() == buffers and cache.capacity == 160
+    assert cache.sync_lengths() == lens and cache.device_status() == 0

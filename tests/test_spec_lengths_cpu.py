@@ -44,3 +44,29 @@ def test_selection_helpers_refuse_sequences_without_tokens():
         cache.estimate_page_criticality(q, exclude_last_page=True)
     with pytest.raises(ValueError, match="no token"):
         cache.select_gaussian_aware(q)
+
+
+@pytest.mark.parametrize("layout", ["dense", "pool"])
+@pytest.mark.parametrize("unseen", ["counts on the device", "replays"])
+def test_a_bound_that_leaves_no_room_is_made_exact_first(layout, unseen, monkeypatch):
+    """Every call may add eight tokens and adds one: neither is the cache copied into a larger one, nor does the pool seem
+    used up, until the tokens are there."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    kw = dict(block_table=True, num_blocks=8) if layout == "pool" else {}
+    cache = host_cache([20, 3], capacity=64, **kw)
+    cache._grows_in_graphs = unseen == "replays"
+    grown = []
+    cache.reserve = grown.append
+    for step in range(30):
+        cache._lens_exact = unseen == "replays"
+        cache._host_lens = cache._room_for(lambda lens: [n + 8 for n in lens])
+        cache.seq_lens += 1
+        assert all(h >= n for h, n in zip(cache.host_seq_lens, cache.seq_lens.tolist())) and not grown, step
+    cache.seq_lens += 30
+    cache._lens_exact = False
+    if layout == "pool":
+        with pytest.raises(RuntimeError, match="may not suffice"):
+            cache._room_for(lambda lens: [n + 8 for n in lens])
+    cache.num_blocks = None
+    cache._room_for(lambda lens: [n + 8 for n in lens])
+    assert len(grown) == 1
