@@ -385,9 +385,8 @@ class PagedKVCache:
                     return_blocks(held, start, self._table, self._free, self.page_size, status=self._ctl)
                     held = torch.minimum(held, start.clamp(min=0))
                 # (only what will be written is planned for: the pool's top follows from the lengths)
-                if counts_host is None:
-                    counts = counts.clamp(max=T)
-                self._plan(held, T if counts is None else counts, status=self._ctl)
+                more = T if counts is None else counts if counts_host is not None else counts.clamp(max=T)
+                self._plan(held, more, status=self._ctl)
             _lib.check(_lib.load().ekv_extend(
                 C.byref(self.desc()), k_new.data_ptr(), v_new.data_ptr(), s[0], s[1], s[2], T, _lib.ptr(counts),
                 _lib.ptr(index), index.stride(0) if index is not None and B > 1 else T, _lib.ptr(start),

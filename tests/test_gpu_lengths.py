@@ -104,3 +104,14 @@ def test_the_loop_runs_as_long_as_its_tokens_fit(layout):
         assert torch.equal(cache.k_cache[0, :, lens[0] - 1], k[0, :, take[0] - 1])
     assert cache._meta.data_ptr() == buffers and cache.capacity == 160
     assert cache.sync_lengths() == lens and cache.device_status() == 0
+
+
+@pytest.mark.parametrize("layout", ["dense", "pool"])
+@pytest.mark.parametrize("counts,start,lens", [([5, 2], None, [43, 35]), ([-1, 3], None, [40, 36]), ([1, 1], [99, 3], [41, 4]),
+                                               ([1, 1], [-2, 3], [1, 4])])
+def test_what_is_clipped_shows_in_the_status(layout, counts, start, lens):
+    cache = make(layout, [40, 33])
+    i32 = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    k = rows(2, 2, 3, 128, seed=5)
+    cache.extend(k, k, counts=i32(counts), start=i32(start))
+    assert cache.device_status() == 4 and cache.sync_lengths() == lens
