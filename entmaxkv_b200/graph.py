@@ -126,6 +126,7 @@ class DecodeStepGraph:
                     cache._host_lens, cache._may_be_empty = list(lens), True
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
+        held = cache._held_by_graphs     # (this graph is captured again when the cache has grown)
         g = torch.cuda.CUDAGraph()
         # a step that holds a collective (``sigma_mean`` given as a callable) is captured in
         # thread-local mode: the process group's watchdog thread keeps polling while this one captures
@@ -138,7 +139,7 @@ class DecodeStepGraph:
             self._call(append=True, out=self._out_alias if with_io else None)
             if with_io and self._out_alias is None:        # no alias of the host buffer: copy the output back
                 self._pinned["out"].copy_(self.out, non_blocking=True)
-        cache._host_lens = lens          # the capture itself appended nothing
+        cache._host_lens, cache._held_by_graphs = lens, held         # the capture itself appended nothing
         if with_io:
             self.graph_io, self._captured_capacity_io = g, cache.capacity
         else:

@@ -68,6 +68,7 @@ class PagedKVCache:
         self._longest = (None, 0)              # (a _host_lens, its largest)
         self._lens_exact = True                # False: device lengths may be below the host's
         self._grows_in_graphs = False          # True: tokens are added by captured calls, whose replays the host does not see
+        self._held_by_graphs = False           # True: a user's graph replays calls on the present buffers
         self._may_be_empty = False             # True: a sequence may hold no token (released, or rewound to 0)
         self._ctl = None                       # int32: [0]=status, [16:16+B] append tickets
         self.last_num_selected_per_head = None
@@ -224,7 +225,7 @@ class PagedKVCache:
             self._k[:, :, :S].copy_(k)
             self._v[:, :, :S].copy_(v)
         self._host_lens = lens
-        self._lens_exact, self._may_be_empty = True, False
+        self._lens_exact, self._may_be_empty, self._held_by_graphs = True, False, False
         self.seq_lens = torch.tensor(lens, dtype=torch.int32, device=k.device)
         self._ctl = torch.zeros(16 + B, dtype=torch.int32, device=k.device)
         self._scratch = {}
@@ -265,12 +266,19 @@ class PagedKVCache:
         return out
 
     def reserve(self, capacity: int):
-        """Grow the buffers so that ``capacity`` rows fit (copies the cache once)."""
+        """Grow the buffers so that ``capacity`` rows fit (copies the cache once).
+
+        Calls captured into a graph keep the addresses of the buffers that they were captured with: after a ``reserve``
+        that grows them (or an ``initialize``) such graphs must not be replayed, only captured again.  While graphs of
+        ``extend`` or ``tree_attention_decode`` exist, the cache does not grow by itself but raises RuntimeError."""
         if self._k is None:
             self._requested_capacity = capacity
             return
         if capacity <= self.capacity:
             return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the cache cannot grow in a captured call: reserve() room before the capture")
+        self._held_by_graphs = False
         B, H, _, D = self._k.shape
         old_k, old_v, old_meta, S = self._k, self._v, self._meta, self.seq_len
         old_pools = (self._pool_k, self._pool_v)
@@ -336,7 +344,8 @@ class PagedKVCache:
         pass ``max_seq_len`` or to call ``sync_lengths`` now and then.  Where the bound leaves no room in the buffers or in
         the pool, the call reads the lengths itself (one synchronisation) before it grows the cache or gives up.
         Values out of range are clipped on the device and show in ``device_status``.
-        ``k_new`` and ``v_new`` must not be views of the cache itself.
+        ``k_new`` and ``v_new`` must not be views of the cache itself.  A call may be captured into a graph, with ``counts``
+        and ``start`` on the device and ``reserve`` called first: its replays write into the buffers of the capture.
         """
         if self._k is None:
             raise RuntimeError("initialize() the cache before extend()")
@@ -378,6 +387,7 @@ class PagedKVCache:
             bound = self._room_for(after)
             capturing = torch.cuda.is_current_stream_capturing()
             self._grows_in_graphs |= capturing
+            self._held_by_graphs |= capturing
             if self.num_blocks is not None:
                 held = self.seq_lens
                 if start is not None:          # what lies behind the rewind goes back first
@@ -420,6 +430,9 @@ class PagedKVCache:
                 "" if self._lens_exact else ", or call sync_lengths() (the host knows only upper bounds of the lengths)"))
         most = max(lens)
         if most > self.capacity:
+            if self._held_by_graphs:
+                raise RuntimeError(f"no room for {most} tokens: captured calls hold the cache's buffers, which therefore do not "
+                                   "grow by themselves; reserve() more and capture again")
             self.reserve(max(most, self.capacity + 4096, self.capacity * 5 // 4))
 
     def _row_lens(self, value, name, most):

@@ -38,6 +38,7 @@ def tree_attention_decode(q: torch.Tensor, kv_cache: PagedKVCache, k_draft: torc
     no longer moves; ``out = sum p v``, written in place and returned.  A row that sees nothing gets zeros and
     ``tau = +inf``; a NaN or +inf score makes its row NaN (output and threshold), a score of -inf is as if unseen.  ``taus_out`` (fp32 [B, H_q, T], contiguous) receives the
     thresholds.  Works on dense and block-table caches; the cache is not changed.  ``out`` must not overlap the inputs.
+    A call may be captured into a graph, after ``kv_cache.reserve``: its replays read the buffers of the capture.
     Scratch comes from torch's allocator in each call: about 8 bytes per row and cached token (of the capacity, where the
     call is captured or captured calls add tokens), at most 6 GiB: then groups of rows take turns.  Little of it is touched.
     """
@@ -79,7 +80,9 @@ def tree_attention_decode(q: torch.Tensor, kv_cache: PagedKVCache, k_draft: torc
         q, k_draft, v_draft = _rows(q), _rows(k_draft), _rows(v_draft)
         # a captured call is replayed while the sequences grow, and replayed appends grow them unseen by the host: then
         # the call is sized by the capacity
-        unseen = kv_cache._grows_in_graphs or torch.cuda.is_current_stream_capturing()
+        capturing = torch.cuda.is_current_stream_capturing()
+        kv_cache._held_by_graphs |= capturing
+        unseen = kv_cache._grows_in_graphs or capturing
         bound = kv_cache.capacity if unseen else min(kv_cache.seq_len, kv_cache.capacity)
         desc = C.byref(kv_cache.desc())
         # scratch of this call alone, from torch's stream-ordered allocator: two streams or two graphs never share it

@@ -115,3 +115,58 @@ def test_what_is_clipped_shows_in_the_status(layout, counts, start, lens):
     k = rows(2, 2, 3, 128, seed=5)
     cache.extend(k, k, counts=i32(counts), start=i32(start))
     assert cache.device_status() == 4 and cache.sync_lengths() == lens
+
+
+def captured(call):
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    return graph
+
+
+@pytest.mark.parametrize("layout", ["dense", "pool"])
+@pytest.mark.parametrize("what", ["extend", "tree"])
+def test_buffers_of_captured_calls_are_not_replaced_unasked(layout, what):
+    """An eager call that has no room raises while a graph holds the buffers; the graph's replays stay right; after
+    reserve() the cache grows by itself again."""
+    import entmaxkv_b200 as E
+    cache = make(layout, [60, 33], capacity=80)
+    k = rows(2, 2, 4, 128, seed=6)
+    counts = torch.tensor([2, 1], dtype=torch.int32, device="cuda")
+    q, mask = rows(2, 4, 4, 128, seed=7), torch.ones(4, 4, dtype=torch.bool, device="cuda").tril()
+    out = torch.zeros_like(q)
+    tree = lambda to: E.tree_attention_decode(q, cache, k, k, mask, to)  # noqa: E731
+    tree(out)
+    graph = captured((lambda: cache.extend(k, k, counts=counts)) if what == "extend" else lambda: tree(out))
+    buffers = cache._meta.data_ptr()
+    many = rows(2, 2, 30, 128, seed=8)
+    with pytest.raises(RuntimeError, match="captured calls hold"):
+        cache.extend(many, many)
+    assert cache._meta.data_ptr() == buffers and cache.seq_lens.tolist() == [60, 33]
+    graph.replay()
+    if what == "extend":
+        assert cache.sync_lengths() == [62, 34]
+        assert torch.equal(cache.k_cache[0, :, 60:62], k[0, :, :2]) and torch.equal(cache.k_cache[1, :, 33], k[1, :, 0])
+    else:
+        want = torch.zeros_like(out)
+        tree(want)
+        assert (out == want).float().mean() > 0.99
+    cache.reserve(100)                               # whoever asks for it knows that the graph is gone
+    cache.extend(many, many)
+    many = rows(2, 2, 4000, 128, seed=9)
+    if layout == "dense":
+        cache.extend(many, many)
+    assert cache.device_status() == 0
+
+
+def test_a_capture_cannot_grow_the_cache():
+    cache = make("dense", [60, 33], capacity=64)
+    many = rows(2, 2, 30, 128, seed=8)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="reserve"):
+        with torch.cuda.graph(graph):
+            cache.extend(many, many)
+    cache.extend(many, many)
+    assert cache.sync_lengths() == [90, 63]
