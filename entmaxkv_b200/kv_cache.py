@@ -280,7 +280,8 @@ class PagedKVCache:
             raise RuntimeError("the cache cannot grow in a captured call: reserve() room before the capture")
         self._held_by_graphs = False
         B, H, _, D = self._k.shape
-        old_k, old_v, old_meta, S = self._k, self._v, self._meta, self.seq_len
+        old_k, old_v, old_meta = self._k, self._v, self._meta
+        S = self.capacity if self._grows_in_graphs else self.seq_len     # (replays add rows that the host does not count)
         old_pools = (self._pool_k, self._pool_v)
         self._allocate(B, H, D, capacity, old_k.dtype, old_k.device)
         if self.num_blocks is not None:

@@ -170,3 +170,24 @@ def test_a_capture_cannot_grow_the_cache():
             cache.extend(many, many)
     cache.extend(many, many)
     assert cache.sync_lengths() == [90, 63]
+
+
+@pytest.mark.parametrize("layout", ["dense", "blocks", "pool"])
+def test_reserve_keeps_rows_that_replays_added(layout):
+    """The host counts no replays: the rows that they wrote must come along when the buffers grow."""
+    import entmaxkv_b200 as E
+    if layout == "blocks":
+        cache = E.PagedKVCache(16, capacity=96, block_table=True, block_order="random")
+        cache.initialize(rows(2, 2, 40, 128, seed=1), rows(2, 2, 40, 128, seed=2), seq_lens=[40, 33])
+    else:
+        cache = make(layout, [40, 33], capacity=96)
+    k, counts = rows(2, 2, 4, 128, seed=6), torch.tensor([4, 3], dtype=torch.int32, device="cuda")
+    graph = captured(lambda: cache.extend(k, k, counts=counts))
+    for _ in range(10):
+        graph.replay()
+    cache.reserve(500)
+    assert cache.sync_lengths() == [80, 63] and cache.capacity >= 500
+    for b, (n0, n) in enumerate(((40, 4), (33, 3))):
+        for view in (cache.k_cache, cache.v_cache):
+            assert torch.equal(view[b, :, n0:n0 + 10 * n], k[b, :, :n].repeat(1, 10, 1))
+    assert cache.device_status() == 0
