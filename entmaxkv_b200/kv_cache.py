@@ -446,6 +446,8 @@ class PagedKVCache:
             if value.dtype != torch.int32 or value.shape != (B,) or not value.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous int32 [{B}] tensor")
             return None, value
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError(f"{name} must be an int32 CUDA tensor in a captured call (a list is copied at each call)")
         host = [int(x) for x in value]
         if len(host) != B or min(host) < 0 or (most is not None and max(host) > most):
             raise ValueError(f"{name} must hold one length per sequence" + (f", at most {most}" if most is not None else ""))
@@ -471,6 +473,8 @@ class PagedKVCache:
             raise ValueError(f"rows must lie in [0, {B})")
         if not rows:
             return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("release() belongs between captured calls, not into them")
         keep = self.seq_lens.clone()
         keep[torch.tensor(rows, device=keep.device)] = 0
         if self.num_blocks is not None:

@@ -191,3 +191,15 @@ def test_reserve_keeps_rows_that_replays_added(layout):
         for view in (cache.k_cache, cache.v_cache):
             assert torch.equal(view[b, :, n0:n0 + 10 * n], k[b, :, :n].repeat(1, 10, 1))
     assert cache.device_status() == 0
+
+
+def test_lists_of_lengths_and_releases_do_not_go_into_captures():
+    cache = make("dense", [40, 33])
+    k = rows(2, 2, 4, 128, seed=6)
+    for call, error in ((lambda: cache.extend(k, k, counts=[1, 2]), ValueError),
+                        (lambda: cache.extend(k, k, start=[1, 2]), ValueError), (lambda: cache.release([0]), RuntimeError)):
+        torch.cuda.synchronize()
+        with pytest.raises(error, match="captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    assert cache.seq_lens.tolist() == [40, 33] and cache.host_seq_lens == [40, 33] and not cache._may_be_empty
