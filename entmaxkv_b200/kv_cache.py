@@ -366,6 +366,12 @@ class PagedKVCache:
         counts_host, counts = self._row_lens(counts, "counts", T)
         start_host, start = self._row_lens(start, "start", None)
 
+        if max_seq_len is not None and self._lens_exact and not self._grows_in_graphs:
+            known = self._host_lens if start is None else [0] * B if start_host is None else start_host
+            known = known if counts_host is None else [n + m for n, m in zip(known, counts_host)]
+            if max(known) > max_seq_len:
+                raise ValueError(f"a sequence will hold {max(known)} tokens, more than max_seq_len = {max_seq_len}")
+
         def after(lens):
             lens = lens if start_host is None else [min(s, n) for s, n in zip(start_host, lens)]
             lens = [n + T for n in lens] if counts_host is None else [n + m for n, m in zip(lens, counts_host)]

@@ -203,3 +203,17 @@ def test_lists_of_lengths_and_releases_do_not_go_into_captures():
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
                 call()
     assert cache.seq_lens.tolist() == [40, 33] and cache.host_seq_lens == [40, 33] and not cache._may_be_empty
+
+
+def test_a_maximum_below_what_is_known_is_refused():
+    cache = make("dense", [40, 33])
+    k = rows(2, 2, 4, 128, seed=6)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for change in (dict(counts=[1, 2], max_seq_len=40), dict(max_seq_len=43), dict(counts=i32(0, 0), max_seq_len=39),
+                   dict(counts=[4, 0], start=[40, 0], max_seq_len=43)):
+        with pytest.raises(ValueError, match="max_seq_len"):
+            cache.extend(k, k, **change)
+    assert cache.host_seq_lens == [40, 33] and cache.seq_lens.tolist() == [40, 33]
+    cache.extend(k, k, counts=[1, 2], max_seq_len=41)
+    cache.extend(k, k, counts=i32(1, 0), start=i32(5, 6), max_seq_len=6)
+    assert cache.sync_lengths() == [6, 6]
