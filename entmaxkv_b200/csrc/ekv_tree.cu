@@ -67,6 +67,8 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
           a.by_page.divmod(key, page, in_page);
           if (kv_page_offset(a.c, b, hkv, page, off))
             raw = ld_stream(static_cast<const T*>(a.c.k) + off + (size_t)in_page * D + e);
+          else if (a.status)
+            atomicOr(a.status, EKV_STATUS_PAGE_RANGE);
         }
         unpack<T>(raw, x);
 #pragma unroll

@@ -387,9 +387,12 @@ __global__ void __launch_bounds__(kTmThreads, 1)
           if (a.c.block_table) {
             int page;
             a.by_page.divmod(key, page, row);
-            // outside the pool, or behind the sequence: zeros
+            // behind the sequence, or (reported) outside the pool: zeros
             block = key < len ? a.c.block_table[(int64_t)b * a.c.bt_stride + page] : -1;
-            if ((unsigned)block >= (unsigned)a.c.num_blocks) block = a.c.num_blocks;
+            if ((unsigned)block >= (unsigned)a.c.num_blocks) {
+              block = a.c.num_blocks;
+              if (key < len && a.status) atomicOr(a.status, EKV_STATUS_PAGE_RANGE);
+            }
           }
           tm_copy_box(smem_addr(s_k) + stage.at * kTileBytes + x * (kTreeTile * 128) + in_tile * 128, &k_map, x * 64,
                       row, hkv, block, &s->full[stage.at]);

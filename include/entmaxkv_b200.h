@@ -324,7 +324,8 @@ int ekv_tau_clamp(const float* tau_hat, int64_t tau_hat_stride, const float* cap
  * k_draft / v_draft [B, H_kv, tokens, D].  z = (alpha-1)/sqrt(D) q.k; tau is the converged root of
  * sum (z - tau)_+^(1/(alpha-1)) = 1 and out = sum (z - tau)_+^(1/(alpha-1)) v.  A row that sees nothing gets
  * zeros and tau = +inf, one with a NaN or +inf score NaN (a score of -inf is as if unseen); rows t >= draft_lens[b] of out and tau stay as
- * they were.  The cache is only read.  Strides {batch, head, token} in elements; tau [B, H_q, tokens]
+ * they were.  The cache is only read; a page whose block lies outside the pool counts as keys and values of zeros and
+ * sets EKV_STATUS_PAGE_RANGE.  Strides {batch, head, token} in elements; tau [B, H_q, tokens]
  * contiguous, may be null.  max_seq_len: host-side upper bound of seq_lens[], at most the capacity (longer
  * sequences are cut to it).  The workspace needs no initialisation; its size grows with rows * max_seq_len
  * up to 6 GiB, then the (sequence, KV head) groups, and the rows of a group that needs more, take turns.

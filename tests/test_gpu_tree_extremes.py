@@ -136,3 +136,21 @@ def test_rows_of_one_group_take_turns():
     assert (whole[0].float() - half[0].float()).abs().max() <= 2 * 2.0 ** -8 * half[0][:, :, :201].float().abs().max()
     assert (whole[0] == half[0]).float().mean() > 0.99
     assert (whole[1] - half[1]).abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("n", [300, 9000])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_a_page_without_a_block_counts_as_zeros_and_is_reported(dt, n):
+    """Table entries outside the pool, which a caller of the C entry point may hand in: the copies and the loads check them."""
+    x = G.make(1, 4, 2, 64, [n], 3, G.DT[dt], seed=55)
+    cache = G.cache_of(x, [n], 16, "blocks")
+    for page, block in ((2, -1), (7, 10 ** 6), (n // 16, 2 ** 31 - 1)):
+        cache._table[0, page] = block
+        for t in (x["k"], x["v"]):
+            t[:, :, 16 * page:16 * page + 16] = 0
+    want = G.run(x, G.cache_of(x, [n], 16, "blocks"), 1.5)
+    import entmaxkv_b200 as E
+    out, tau = torch.zeros_like(x["q"]).cuda(), torch.zeros(x["q"].shape[:3], device="cuda")
+    E.tree_attention_decode(x["q"].cuda(), cache, x["kd"].cuda(), x["vd"].cuda(), x["mask"].cuda(), out, taus_out=tau)
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(tau.cpu(), want[1])
+    assert cache.device_status() == 1
