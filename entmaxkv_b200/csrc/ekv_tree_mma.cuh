@@ -66,17 +66,20 @@ __device__ __forceinline__ bool tm_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok;
 }
-__device__ __forceinline__ void tm_wait(uint64_t* bar, uint32_t parity, TmSmem* s, int* status) {
+// false: a wait of the block ran out.  From then on nothing more is copied, the other waits end at once, and the launch's
+// results are undefined (the status says so).
+__device__ __forceinline__ bool tm_wait(uint64_t* bar, uint32_t parity, TmSmem* s, int* status) {
   const uint32_t b = smem_addr(bar);
-  if (tm_try(b, parity)) return;
+  if (tm_try(b, parity)) return true;
   const long long start = clock64();
   while (!tm_try(b, parity)) {
-    if (*(volatile int*)&s->abort) return;
-    if (clock64() - start > (1ll << 32)) {       // some two seconds: a wait that ran out ends all others of the block
+    if (*(volatile int*)&s->abort) return false;
+    if (clock64() - start > (1ll << 32)) {       // some two seconds
       *(volatile int*)&s->abort = 1;
       note_copy_timeout(status);
     }
   }
+  return true;
 }
 // a place in a ring of `size` barriers and the parity of its current turn
 struct TmRing {
@@ -264,7 +267,8 @@ __global__ void __launch_bounds__(kTmThreads, 1)
   TmRing stage, acc_ring;
   int n = 0;                                               // tiles so far
   int segment = 0;
-  for (int g = at.g; g < a.g1 && g_first < t_end; ++g) {
+  bool go = true;                                          // (copies only) no wait ran out
+  for (int g = at.g; g < a.g1 && g_first < t_end && go; ++g) {
     const int b = g / H, hkv = g % H;
     const int g_tiles = tree_tiles<SAMPLE>(a, b);
     if (g_tiles == 0) continue;
@@ -377,9 +381,10 @@ __global__ void __launch_bounds__(kTmThreads, 1)
       const int boxes = a.tile_keys / sh.box_rows * KB;
       for (int tile = tile0; tile < tile1; ++tile, ++n) {
         const int place = SAMPLE ? tree_sample_tile(tile, g_tiles, all_tiles) : tile;
-        if (n >= sh.stages) tm_wait(&s->empty[stage.at], stage.parity ^ 1, s, a.status);
-        if (first_box == 0) mbar_expect_tx(&s->full[stage.at], (uint32_t)a.tile_keys * D * 2);
-        __syncwarp();
+        if (n >= sh.stages) go = tm_wait(&s->empty[stage.at], stage.parity ^ 1, s, a.status);
+        if (first_box == 0 && go) mbar_expect_tx(&s->full[stage.at], (uint32_t)a.tile_keys * D * 2);
+        go = __all_sync(0xffffffffu, go);
+        if (!go) break;
         for (int i = first_box; i < boxes; i += 32 * kTmCopyWarps) {
           const int in_tile = i / KB * sh.box_rows, x = i % KB;
           const int key = place * a.tile_keys + in_tile;
@@ -440,6 +445,9 @@ __global__ void __launch_bounds__(kTmThreads, 1)
       }
     __syncwarp();
   }
+  // after a wait that ran out: copies and products on their way still use this block's memory, so it stays some 8 ms longer
+  if (warp >= kTmEpiWarps && *(volatile int*)&s->abort)
+    for (const long long start = clock64(); clock64() - start < (1ll << 24);) __nanosleep(1000);
   if (MODE == TM_LISTS) tree_wait_for_previous();
   tm_fence_before();
   __syncthreads();
