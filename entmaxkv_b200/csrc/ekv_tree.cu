@@ -487,9 +487,10 @@ __device__ void fin_block_row(const TreeArgs& a, const FinRow& r, uint2* s_slots
     if (w > 0.f) rows.put(at, make_uint2(__float_as_uint(w), (uint32_t)fin_pool_key(a, r, (int)e.y)));
     m += total;
   }
-  // alpha > 2: keys next to the root weigh (rounding)^beta, and no tau that fp32 holds makes thousands of them sum to one
+  // far from alpha 1.5 and 2 a power makes much of a rounding: above 2 keys next to the root weigh (rounding)^beta, near 1
+  // every weight is off by beta roundings, and no tau that fp32 holds makes them sum to one
   sum_w = block_sum(sum_w, scratch);
-  const float scale = beta < 1.f ? 1.f / sum_w : 1.f;
+  const float scale = kind == 2 ? 1.f / sum_w : 1.f;
   float acc[EPL] = {};
   const int sub = tid / LPR, col = tid % LPR * EPL;
   for (int i0 = sub; i0 < m; i0 += GROUPS * N) {
@@ -717,9 +718,8 @@ __global__ void __launch_bounds__(kFinWarps * 32, 7) tree_finish_kernel(const __
       for (int o = LPR; o < 32; o <<= 1)
 #pragma unroll
         for (int j = 0; j < EPL; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
-      // alpha > 2: keys next to the root weigh (rounding)^beta, and no tau that fp32 holds makes thousands of them sum to one
       sum_w = warp_sum(sum_w);
-      const float scale = beta < 1.f ? 1.f / sum_w : 1.f;
+      const float scale = kind == 2 ? 1.f / sum_w : 1.f;         // see fin_block_row
       if (lane < LPR)
 #pragma unroll
         for (int j = 0; j < EPL; ++j) out[col + j] = from_float<T>(acc[j] * scale);

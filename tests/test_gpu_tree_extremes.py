@@ -63,7 +63,7 @@ def level_scores(dt, n, shape, alpha, score):
     return x
 
 
-@pytest.mark.parametrize("alpha", [1.5, 2.0, 3.0])
+@pytest.mark.parametrize("alpha", [1 + 2.0 ** -11, 1.125, 1.5, 2.0, 3.0, 5.0])
 @pytest.mark.parametrize("dt,n,shape", PLACES)
 def test_weights_of_equal_scores_sum_to_one(dt, n, shape, alpha):
     """n + 1 equal scores of 8 and values of one: the output is the sum of the weights.  The solver leaves it within
