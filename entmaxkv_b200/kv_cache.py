@@ -457,8 +457,12 @@ class PagedKVCache:
         host = [int(x) for x in value]
         if len(host) != B or min(host) < 0 or (most is not None and max(host) > most):
             raise ValueError(f"{name} must hold one length per sequence" + (f", at most {most}" if most is not None else ""))
-        if most is None and self._lens_exact and any(s > n for s, n in zip(host, self._host_lens)):
-            raise ValueError(f"{name} lies beyond the sequence's length")
+        beyond = lambda: any(s > n for s, n in zip(host, self._host_lens))  # noqa: E731
+        if most is None and beyond():
+            if self._grows_in_graphs:              # replays may have added what the host does not know of
+                self.sync_lengths()
+            if self._lens_exact and beyond():
+                raise ValueError(f"{name} lies beyond the sequence's length")
         return host, torch.tensor(host, dtype=torch.int32, device=device)
 
     def sync_lengths(self) -> list[int]:

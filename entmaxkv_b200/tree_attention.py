@@ -36,8 +36,9 @@ def tree_attention_decode(q: torch.Tensor, kv_cache: PagedKVCache, k_draft: torc
 
     ``p = ((alpha-1) q.k / sqrt(D) - tau)_+^(1/(alpha-1))`` with the tau that makes each row sum to one, solved until it
     no longer moves; ``out = sum p v``, written in place and returned.  A row that sees nothing gets zeros and
-    ``tau = +inf``; a NaN or +inf score makes its row NaN (output and threshold), a score of -inf is as if unseen.  ``taus_out`` (fp32 [B, H_q, T], contiguous) receives the
-    thresholds.  Works on dense and block-table caches; the cache is not changed.  ``out`` must not overlap the inputs.
+    ``tau = +inf``; a NaN or +inf score makes its row NaN (output and threshold), a score of -inf is as if unseen.
+    ``taus_out`` (fp32 [B, H_q, T], contiguous) receives the thresholds.  Works on dense and block-table caches; the cache
+    is not changed.  ``out`` must not overlap the inputs.
     A call may be captured into a graph, after ``kv_cache.reserve``: its replays read the buffers of the capture.
     Scratch comes from torch's allocator in each call: about 8 bytes per row and cached token (of the capacity, where the
     call is captured or captured calls add tokens), at most 6 GiB: then groups of rows take turns.  Little of it is touched.

@@ -217,3 +217,20 @@ def test_a_maximum_below_what_is_known_is_refused():
     cache.extend(k, k, counts=[1, 2], max_seq_len=41)
     cache.extend(k, k, counts=i32(1, 0), start=i32(5, 6), max_seq_len=6)
     assert cache.sync_lengths() == [6, 6]
+
+
+def test_a_rewind_among_rows_that_replays_added():
+    """The host counts one call of a captured extend, three replays wrote: a start between the two is no mistake, one
+    beyond the tokens is."""
+    cache = make("dense", [40, 33], capacity=96)
+    k = rows(2, 2, 4, 128, seed=6)
+    graph = captured(lambda: cache.extend(k, k))
+    for _ in range(3):
+        graph.replay()
+    with pytest.raises(ValueError, match="beyond"):
+        cache.extend(k, k, start=[53, 40])
+    for _ in range(3):
+        graph.replay()                                                   # 64 and 57 tokens, 52 and 45 of them known
+    cache.extend(k, k, start=[61, 50], counts=[2, 0])
+    assert cache.host_seq_lens == [63, 50] == cache.seq_lens.tolist() and cache.device_status() == 0
+    assert torch.equal(cache.k_cache[0, :, 61:63], k[0, :, :2])
