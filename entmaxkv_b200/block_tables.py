@@ -51,7 +51,8 @@ def plan_block_tables(seq_lens: torch.Tensor, new_lens: Union[torch.Tensor, int]
     seq_lens int32 [B]: tokens that each sequence holds, on ``ceil(seq_lens / page_size)`` pages; new_lens int32 [B] or
     one int for all.  ``free_blocks`` int32 [num_blocks] is the pool as a stack: its lowest ``sum(held pages)`` places
     are in use (their content does not matter), and the missing pages take the places from there on in sequence order,
-    -1 once the pool is used up.  A sequence gets no pages behind the table's width.  ``block_table`` int32 [B, pages] gets those entries and keeps the others.
+    -1 once the pool is used up.  A sequence gets no pages behind the table's width.  ``block_table`` int32 [B, pages]
+    gets those entries and keeps the others.
 
     The new tokens of all sequences one after another get ``slots`` (int64: block * page_size + place in the page, -1
     without a block) and ``positions`` (int32), both -1 behind the last token; ``row_starts`` (int32 [B + 1]) says where

@@ -5,8 +5,9 @@
 // and the new ones, 16 on their way at a time - stores the new ones and forms the column's statistics from the same
 // registers, so a new row is read once and written once and an old row is read only where it shares the first page.
 // Values are copied by blocks of their own: with both in one thread the registers leave too few loads in flight.
-// Bound by memory: 8 sequences, 3000 to 4096 rows each, 8 heads of 128, bf16: 56 us, 5.0 TB/s, 0.76 of a plain copy
-// (with a cold cache 59 us, against 61 with 256-thread blocks and 72 with keys and values in one thread).  A tree's accepted path, 32 sequences: 9 us, latency.
+// Bound by memory: 8 sequences, 3000 to 4096 rows each, 8 heads of 128, bf16: 56 us, 5.0 TB/s, 0.76 of a plain copy (a launch
+// alone 54 us; 128-thread blocks took 0.97 of the time of 256-thread blocks, keys and values in one thread 1.22).  A tree's
+// accepted path, 32 sequences: 10 us, latency.
 #include "ekv_page_stats.cuh"
 
 namespace ekv {

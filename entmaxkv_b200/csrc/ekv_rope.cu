@@ -12,10 +12,11 @@
 // stay in registers, the cosines and sines are read once per token, and four rows are on their way while one is worked
 // on.  A block takes several tokens, whose angles it computes first.
 //
-// Measured on a B200: 20,495 tokens of 64 heads of 64, bf16, half rotated: 80 us, 4.2 TB/s, 0.64 of a plain copy (bound by
-// instruction issue: about 85 instructions per 16 bytes, with the products in packed pairs); 512 tokens of 72 heads of
-// 128: 10 us; one token: 4 us.  With a cold cache 84 us, against 88 with 256-thread blocks and 137 with cosines and
-// weights held in registers for all heads (98 registers, two blocks to an SM).
+// Measured on a B200: 20,495 tokens of 64 heads of 64, bf16, half rotated: 80 us, 4.2 TB/s, 0.64 of a plain copy (about 85
+// instructions per 16 bytes, with the products in packed pairs, take 69 % of the issue slots; 64 registers, of which the
+// 16-bit forms spill 8 to 64 bytes, hold eight blocks to an SM); 512 tokens of 72 heads of 128: 10 us; one token: 6 us.
+// 128-thread blocks took 0.95 of the time of 256-thread blocks, and 0.61 of that with cosines and weights held in
+// registers for all heads (98 registers, two blocks to an SM).
 #include "ekv_common.cuh"
 
 namespace ekv {

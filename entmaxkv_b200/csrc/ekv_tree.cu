@@ -7,7 +7,8 @@ namespace ekv {
 
 // ---- scores on the CUDA cores -------------------------------------------------------------------------------------
 //
-// For fp32 caches, which have no tensor-core product of their precision.  A block scores 32 rows against 64 keys at a
+// For fp32 caches, which have no tensor-core product of their precision (8 sequences of 4096 tokens, 32 rows per KV head, 8
+// heads of 128: 230 us the whole call, 8 % of them K's bytes).  A block scores 32 rows against 64 keys at a
 // time: lane = row, warp = eight of the keys, so a key's elements are one broadcast read per warp and each thread owns
 // (row, eight keys of every half tile) with a list of its own.
 constexpr int kSimtRows = 32, kSimtKeys = 64, kSimtWarps = 8;
@@ -116,8 +117,9 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_scores_simt_kernel(const
 // the GPU holds blocks) get a block each from the start.
 //
 // Bound by latency: the chain lists -> entries -> tau (five or six sums) -> value rows of some 40 keys.  4096 rows of 17k to
-// 32k tokens: 30 us alone, of which most lies behind the last tiles of the score pass; 256 rows with all 4096 scores: 20 us
-// with a block each (38 us with a warp each).
+// 32k tokens: 31 us alone, of which most lies behind the last tiles of the score pass; 256 rows with all 4096 scores: 16 us
+// with a block each (a warp each took about twice that).  The threshold relative to the maximum
+// cost 1 to 2 us of a call.
 
 constexpr int kFinWarps = 4;                    // warps of a block that takes a row per warp
 constexpr int kFinOneWarps = 8;                 // and of one that takes a single row

@@ -16,10 +16,11 @@
 // costs.
 //
 // Measured on a B200 (a launch alone): 8 sequences of 17k to 32k tokens, 64 rows per KV head, 8 heads of 128: sample 20 us,
-// pass 80 us, 387 MB at 4.9 TB/s, 1.2k cycles a tile where it streams; one sequence of 131k tokens, 512 rows per KV head
-// (two blocks of rows share each K tile through L2): pass 155 us, 2.4k cycles a tile of 128 keys by 256 rows, 1.0k of them
-// products; the rest is the epilogue's comparisons and appends.  With keys along the lanes instead of rows the same passes
-// took 112 and 280 us.
+// pass 80 us, 387 MB at 4.8 TB/s, 1.2k cycles a tile where it streams; one sequence of 131k tokens, 512 rows per KV head
+// (two blocks of rows share each K tile through L2): pass 172 us.  At half that length 101 us, 137 MB from memory, the tensor
+// pipe 33 % and the issue slots 56 % busy: about 1.7k slots a tile of 128 keys by 256 rows beside 1.0k cycles of products,
+// most of them the epilogue's comparisons and appends.  With keys along the lanes instead of rows the passes took 1.2 and 1.8
+// times as long.
 #pragma once
 
 #include <cuda.h>

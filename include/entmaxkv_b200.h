@@ -143,7 +143,8 @@ int ekv_extend(const ekv_cache_desc* c, const void* k_new, const void* v_new, in
  * [held[b], need[b]) gets block_table[b, p] = free_blocks[sum(held) + sum_{b' < b}(need - held) + p - held[b]],
  * or -1 past the end of the list.  The list is a stack whose lowest sum(held) places are in use: their
  * content does not matter, and the call changes nothing but table entries behind a sequence's held pages,
- * so it can be repeated.  A sequence gets no pages behind the table's width.  The new tokens of all sequences, one after another, get
+ * so it can be repeated.  A sequence gets no pages behind the table's width.  The new tokens of all
+ * sequences, one after another, get
  *   slots[r] = block * page_size + position % page_size (-1 without a block), positions[r] = position,
  * both -1 from the last token on; row_starts[b] (B + 1 entries) is where sequence b's tokens begin.
  * slots, positions, row_starts and status may be null; status gets EKV_STATUS_CAPACITY when the pool or the
@@ -323,8 +324,8 @@ int ekv_tau_clamp(const float* tau_hat, int64_t tau_hat_stride, const float* cap
  * (null: all) with mask[b, t, j] != 0 (bytes; mask_stride_b 0 for one mask), whose keys and values are
  * k_draft / v_draft [B, H_kv, tokens, D].  z = (alpha-1)/sqrt(D) q.k; tau is the converged root of
  * sum (z - tau)_+^(1/(alpha-1)) = 1 and out = sum (z - tau)_+^(1/(alpha-1)) v.  A row that sees nothing gets
- * zeros and tau = +inf, one with a NaN or +inf score NaN (a score of -inf is as if unseen); rows t >= draft_lens[b] of out and tau stay as
- * they were.  The cache is only read; a page whose block lies outside the pool counts as keys and values of zeros and
+ * zeros and tau = +inf, one with a NaN or +inf score NaN (a score of -inf is as if unseen); rows
+ * t >= draft_lens[b] of out and tau stay as they were.  The cache is only read; a page whose block lies outside the pool counts as keys and values of zeros and
  * sets EKV_STATUS_PAGE_RANGE.  Strides {batch, head, token} in elements; tau [B, H_q, tokens]
  * contiguous, may be null.  max_seq_len: host-side upper bound of seq_lens[], at most the capacity (longer
  * sequences are cut to it).  The workspace needs no initialisation; its size grows with rows * max_seq_len
